@@ -1,0 +1,43 @@
+// Entry points of the attention over the 8-bit cache.
+#include "attention_quant_decode.cuh"
+
+namespace edgelm {
+int launch_decode_quant_int8(const QuantDecodeArgs& p, int dtype, int hd, int n_seqs, int n_splits, int warps, cudaStream_t stream);
+int launch_decode_quant_fp8(const QuantDecodeArgs& p, int dtype, int hd, int n_seqs, int n_splits, int warps, cudaStream_t stream);
+}  // namespace edgelm
+
+using namespace edgelm;
+
+// One new token a sequence.  With the position tables (cos_t, sin_t [max_pos, hd / 2]) `q` holds the raw q, k, v projections
+// [n_seqs, (nh + 2 nkv) hd]: the kernel rotates, appends the new rows as codes (kcache, vcache, k_scale, v_scale are written) and
+// attends over the cache with them.  Without: `q` holds rotated query heads and the cache every row up to seq_pos.
+// n_splits: blocks that share a sequence's keys, 1 to 16.  Returns 0 or a negative code.
+extern "C" int edgelm_attn_decode_quantized(const void* q, long long ldq, void* out, long long ldo, void* kcache, void* vcache, float* k_scale,
+                                            float* v_scale, int dtype, int format, const int32_t* page_table, int table_stride, int n_pages,
+                                            const int32_t* seq_slot, const int32_t* seq_pos, const float* cos_t, const float* sin_t, int max_pos,
+                                            int n_seqs, int nh, int nkv, int hd, float scale, int n_splits, int window, int meta_ready, int* err,
+                                            cudaStream_t stream) {
+  if (n_seqs == 0) return 0;
+  const char* who = "attn_decode_quantized";
+  EL_REFUSE(nh > 0 && nkv > 0 && nh % nkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, nh, nkv);
+  EL_REFUSE(hd >= 16 && hd <= 256 && hd % 16 == 0, "%s: head size %d (takes 16..256 in steps of 16)", who, hd);
+  EL_REFUSE((format == QF_INT8 || format == QF_FP8) && (dtype == DT_F32 || dtype == DT_BF16), "%s: format %d, dtype %d", who, format, dtype);
+  EL_REFUSE(n_seqs > 0 && n_seqs <= 65535, "%s: %d sequences (takes up to 65,535)", who, n_seqs);
+  const int chunks = (nh / nkv + QD_HEADS - 1) / QD_HEADS;
+  EL_REFUSE((long long)nkv * chunks <= 65535, "%s: too many heads", who);
+  EL_REFUSE(n_splits >= 1 && n_splits <= QD_MAX_SPLITS, "%s: %d splits (takes 1 to %d)", who, n_splits, QD_MAX_SPLITS);
+  EL_REFUSE(window >= 0, "%s: a window of %d keys", who, window);
+  EL_REFUSE((cos_t == nullptr) == (sin_t == nullptr) && (cos_t == nullptr || max_pos > 0), "%s: position tables", who);
+  EL_REFUSE((uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0 && (uintptr_t)k_scale % 16 == 0 && (uintptr_t)v_scale % 16 == 0,
+            "%s: the cache must start on 16-byte boundaries", who);
+  EL_REFUSE((uintptr_t)out % 8 == 0 && ldo % 2 == 0, "%s: output rows must start on 8-byte boundaries", who);
+  const QuantDecodeArgs p = {q, out, (uint8_t*)kcache, (uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos_t, sin_t, err,
+                             ldq, ldo, table_stride, n_pages, max_pos, nh, nkv, window, meta_ready, scale};
+  // Four warps a block, three blocks an SM; eight warps where the blocks do not go round the SMs, so that as many copies are in flight.
+  const int warps = (long long)n_seqs * nkv * chunks * n_splits <= 148 ? 8 : 4;
+  const int rc = format == QF_INT8 ? launch_decode_quant_int8(p, dtype, hd, n_seqs, n_splits, warps, stream)
+                                   : launch_decode_quant_fp8(p, dtype, hd, n_seqs, n_splits, warps, stream);
+  if (rc) return rc;
+  EL_LAUNCH_CHECK(who);
+  return 0;
+}

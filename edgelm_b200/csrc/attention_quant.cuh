@@ -1,0 +1,89 @@
+// What the attention kernels over the 8-bit cache share: float16 products of codes, and the arithmetic of scores and weights.
+//
+// With codes a (keys) and c (values) and scales u_j, v_j:   out = sum_j p_j v_j c_j / sum_j p_j,   p_j = 2^(s_j - m),
+// s_j = log2(e) scale u_j (q . a_j).  Let v_j = f_j 2^e_j, e_j the float's exponent (held to -40 at least).  The kernels keep
+//     x_j = s_j + e_j,   t_j = 2^(x_j - M + 60),   M >= x_j for all j so far,
+// and sum   w_j c_j  with w_j = t_j f_j 2^-46 (the operand of the product with the codes: a float16 number under 2^15), and t_j 2^-e_j
+// (the same weight without its value's scale, in float32).  A weight is small beside the largest *weighted* row only, whatever the
+// scales of the rows, so no scale pushes the operand out of float16's range: 2^14 keeps 28 bits below the largest weight above
+// float16's smallest number, and rows that are all under 2^-33 have at least 11 (f down to 2^-27).  2^60 is as far from float32's
+// largest number (2^100 a row, with e = -40) as rows that weigh nothing in the sum of values, but count in the other, are from its
+// smallest.  Taking e_j off the float is exact and costs no logarithm.
+//
+// The queries' rows are brought to at most 2^13 by a power of two before they become float16 numbers (28 bits below a row's largest
+// number survive); float32 models carry a second term, x - float16(x), of queries and weights: 22 bits.
+#pragma once
+#include "quant_cache.cuh"
+
+namespace edgelm {
+
+constexpr float AQ_LIFT = 60.f;            // t <= 2^60
+constexpr float AQ_OPERAND = 1.4210854715202004e-14f;   // 2^-46: the largest weight as an operand is 2^14 to 2^15
+constexpr float AQ_OPERAND_BACK = 70368744177664.f;     // 2^46, for the finished sums of values
+constexpr int AQ_QUERY_EXP = 12;           // a query row's largest number lies in [2^12, 2^13)
+constexpr float AQ_LOG2E = 1.4426950408889634f;
+constexpr long long AQ_WAIT_CYCLES = 2000000000LL;
+
+__device__ __forceinline__ uint32_t aq_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float aq_exp2(float x) {   // 2^x on the special-function unit; 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void aq_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t aq_pack(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// the second term of a pair: what float16 left out
+__device__ __forceinline__ uint32_t aq_rest(float lo, float hi, uint32_t first) {
+  const float2 f = half2_to_floats(first);
+  return aq_pack(lo - f.x, hi - f.y);
+}
+__device__ __forceinline__ uint32_t aq_transpose8(uint32_t x) {   // an 8 x 8 matrix of 16-bit values spread over the warp, transposed
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// A value's scale as f 2^e, f with the operand's 2^-46 (f keeps a NaN).
+struct ValueScale {
+  float e, f, undo;    // undo = 2^-e
+};
+__device__ __forceinline__ ValueScale value_scale(float v) {
+  const int b = min(max((int)((__float_as_uint(v) >> 23) & 255u), 127 - 40), 253);
+  const float undo = __uint_as_float((uint32_t)(254 - b) << 23);
+  return {(float)(b - 127), v * undo * AQ_OPERAND, undo};
+}
+
+// The power of two that brings a query row with this largest magnitude into [2^12, 2^13), and what undoes it.  (Rows that are not
+// finite stay so; rows of zeros, or under 2^-100, keep a factor whose inverse is a number.)
+__device__ __forceinline__ float query_lift(uint32_t largest_bits) {
+  const int e = min(max((int)(largest_bits >> 23), 27), 227) - 127;    // floor(log2), held to -100 .. 100
+  return __uint_as_float((uint32_t)(AQ_QUERY_EXP - e + 127) << 23);
+}
+
+// Bounded wait for a phase of an mbarrier: false once the clock says that it will not come.
+__device__ __forceinline__ bool aq_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool aq_wait(uint32_t bar, uint32_t parity) {
+  if (aq_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!aq_try(bar, parity))
+    if (clock64() - t0 > AQ_WAIT_CYCLES) return false;
+  return true;
+}
+__device__ __forceinline__ void aq_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+}  // namespace edgelm

@@ -1539,3 +1539,139 @@ def softcap(z, cap):
     """z <- cap * tanh(z / cap), in place (float32)."""
     _f32(z, "z")
     _check(lib().edgelm_softcap(_p(z), ctypes.c_longlong(z.numel()), ctypes.c_float(cap), _stream()))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# The 8-bit cache (quant_cache.cuh): keys and values as codes [pages, kv_heads, PAGE, head_dim] (torch.int8, or torch.float8_e4m3fn)
+# with a float32 scale a row [pages, kv_heads, PAGE].  A row x is kept as scale = A / top and codes round(x * (top / A)) with
+# A = max(|x_i|, 2^-60) and top 127 (int8) or 448 (e4m3); a row with a number that is not finite has the scale NaN and codes of zero.
+
+QUANT_FORMATS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+QUANT_PREFILL_TILE = 128   # new tokens per tile of the prompt attention over the 8-bit cache
+QUANT_MAX_SPLITS = 16      # blocks that share a sequence's keys in its decode attention (QD_MAX_SPLITS in attention_quant_decode.cuh)
+_QUANT_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+def _entry(name, kinds):
+    """The library's function `name`, taking Python numbers: a letter an argument (p pointer, i int, l long long, f float)."""
+    fn = getattr(lib(), name)
+    if fn.argtypes is None:
+        fn.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}[k] for k in kinds]
+    return fn
+
+
+def _a(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what):
+    """Checks the cache's tensors; the format's code."""
+    code = _QUANT_CODES.get(kcache.dtype)
+    _need(code is not None and vcache.dtype == kcache.dtype, f"{what}: the cache's codes must be int8 or float8_e4m3fn, keys and values alike")
+    shape = kcache.shape
+    _need(len(shape) == 4 and shape[1:] == (nkv, PAGE, hd) and vcache.shape == shape, f"{what}: codes must be [pages, {nkv}, {PAGE}, {hd}]")
+    _need(k_scale.shape == shape[:3] and v_scale.shape == shape[:3] and k_scale.dtype == v_scale.dtype == torch.float32, f"{what}: scales must be float32 [pages, {nkv}, {PAGE}]")
+    _need(kcache.is_contiguous() and vcache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous(), f"{what}: the cache must be contiguous")
+    _need(kcache.is_cuda and kcache.device.index == torch.cuda.current_device(), f"{what}: the cache must lie on the current device")
+    return code
+
+
+def _quant_steps(page_table, tensors, what):
+    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_cuda and page_table.stride(1) == 1, f"{what}: the page table must be int32 rows")
+    for t, name in tensors:
+        _need(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous(), f"{what}: {name} must be a contiguous int32 CUDA tensor")
+
+
+def _quant_tables(cos, sin, hd, what):
+    _need(cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd // 2 and
+          cos.is_contiguous() and sin.is_contiguous() and cos.is_cuda and sin.is_cuda, f"{what}: table layout")
+
+
+def _heads(nh, nkv, hd, what):
+    _need(nh > 0 and nkv > 0 and nh % nkv == 0, f"{what}: {nh} query heads are not a multiple of {nkv} key/value heads")
+    _need(16 <= hd <= 256 and hd % 16 == 0, f"{what}: head size {hd} (takes 16 to 256 in steps of 16)")
+
+
+def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, kcache, vcache, k_scale, v_scale, nh, nkv, hd, err):
+    """`rope_kv_append` into the 8-bit cache: rotate q and k of the fused projection output in float32 (q back in place), write k and v
+    as codes and scales into their pages."""
+    what = "rope_quantize_append"
+    _heads(nh, nkv, hd, what)
+    T = qkv.shape[0]
+    _need(qkv.is_contiguous() and qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * hd, f"{what}: qkv layout")
+    code = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    _quant_tables(cos, sin, hd, what)
+    _quant_steps(page_table, ((tok_pos, "tok_pos"), (tok_seq, "tok_seq"), (seq_slot, "seq_slot"), (err, "err")), what)
+    _need(tok_pos.numel() >= T and tok_seq.numel() >= T, f"{what}: one position and one sequence index per token")
+    _check(_entry("edgelm_rope_quantize_append", "piipppp" "iippi" "pppp" "iiiipp")(
+        _a(qkv), _dt(qkv), code, _a(tok_pos), _a(tok_seq), _a(seq_slot), _a(page_table), page_table.stride(0), kcache.shape[0], _a(cos), _a(sin),
+        cos.shape[0], _a(kcache), _a(vcache), _a(k_scale), _a(v_scale), T, nh, nkv, hd, _a(err), torch.cuda.current_stream().cuda_stream),
+        launches=1 if T else 0)
+
+
+def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot, page_table, keys, values, err):
+    """keys[t], values[t] = what the 8-bit cache holds for token t (position tok_pos[t] of sequence tok_seq[t]): [T, kv_heads, head_dim],
+    float32 or bfloat16, code * scale in float32 rounded once.  A token whose page the cache does not have: zeros, and a bit of `err`."""
+    what = "quantized_rows"
+    _need(keys.dim() == 3 and keys.shape == values.shape and keys.dtype == values.dtype and keys.is_contiguous() and values.is_contiguous() and keys.is_cuda, f"{what}: rows must be contiguous [tokens, kv_heads, head_dim]")
+    T, nkv, hd = keys.shape
+    _heads(nkv, nkv, hd, what)
+    code = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    _quant_steps(page_table, ((tok_pos, "tok_pos"), (tok_seq, "tok_seq"), (seq_slot, "seq_slot"), (err, "err")), what)
+    _need(tok_pos.numel() >= T and tok_seq.numel() >= T, f"{what}: one position and one sequence index per token")
+    _check(_entry("edgelm_quantized_rows", "ppppi" "ppppii" "ppi" "iiipp")(
+        _a(kcache), _a(vcache), _a(k_scale), _a(v_scale), code, _a(tok_pos), _a(tok_seq), _a(seq_slot), _a(page_table), page_table.stride(0),
+        kcache.shape[0], _a(keys), _a(values), _dt(keys), T, nkv, hd, _a(err), torch.cuda.current_stream().cuda_stream), launches=1 if T else 0)
+
+
+def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
+    """Blocks that share a sequence's keys in the decode attention over the 8-bit cache: enough for two an SM, as long as each of a
+    block's four warps can get a tile of keys (64, 32 or 16 by head size)."""
+    tile = 64 if hd <= 64 else 32 if hd <= 128 else 16
+    blocks = max(1, n_seqs * nkv * -(-(nh // nkv) // 8))
+    splits = 1
+    while splits < QUANT_MAX_SPLITS and blocks * splits < 2 * n_sms and 4 * tile * splits < max_keys:
+        splits *= 2
+    return splits
+
+
+def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv, hd, scale, n_splits,
+                           err, window, meta_ready):
+    _heads(nh, nkv, hd, what)
+    _need(q.dtype == out.dtype and q.dim() == 2 and out.dim() == 2 and q.stride(1) == 1 and out.stride(1) == 1, f"{what}: rows must be contiguous, of one type")
+    width = nh * hd if cos is None else (nh + 2 * nkv) * hd
+    _need(q.shape[0] >= n_seqs and out.shape[0] >= n_seqs and q.shape[1] >= width and out.shape[1] >= nh * hd and out.is_cuda and q.is_cuda, f"{what}: shapes")
+    code = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    _quant_steps(page_table, ((seq_slot, "seq_slot"), (seq_pos, "seq_pos")) + (((err, "err"),) if err is not None else ()), what)
+    _need(seq_slot.numel() >= n_seqs and seq_pos.numel() >= n_seqs, f"{what}: one slot and one position per sequence")
+    window = int(window or 0)
+    if n_splits is None:
+        keys = page_table.shape[1] * PAGE
+        n_splits = quantized_decode_splits(n_seqs, nh, nkv, hd, min(keys, window) if window else keys)
+    max_pos = 0
+    if cos is not None:
+        _quant_tables(cos, sin, hd, what)
+        max_pos = cos.shape[0]
+    _check(_entry("edgelm_attn_decode_quantized", "plplpppp" "iipiipp" "ppi" "iiiif" "iiipp")(
+        _a(q), q.stride(0), _a(out), out.stride(0), _a(kcache), _a(vcache), _a(k_scale), _a(v_scale), _dt(q), code, _a(page_table),
+        page_table.stride(0), kcache.shape[0], _a(seq_slot), _a(seq_pos), _a(cos), _a(sin), max_pos, n_seqs, nh, nkv, hd, scale, n_splits, window,
+        1 if meta_ready else 0, _a(err), torch.cuda.current_stream().cuda_stream), launches=1 if n_seqs else 0)
+
+
+def attn_decode_quantized(q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, n_seqs, nh, nkv, hd, scale, n_splits=None,
+                          err=None, window=0, meta_ready=False):
+    """`attn_decode` over the 8-bit cache: one new token per sequence, its query heads in q [n_seqs, nh * hd (or more)], its key and value
+    in the cache already.  `n_splits`: blocks that share a sequence's keys, 1 to 16 (None: by sizes, with the page table's width as
+    the longest sequence); their results meet on the chip, no scratch is taken.  A sequence with seq_pos < 0 has no token: its row
+    of `out` is zero.  `window`, `err`, `meta_ready`: as in `attn_decode`."""
+    _attn_decode_quantized("attn_decode_quantized", q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, None, None, n_seqs, nh, nkv, hd,
+                           scale, n_splits, err, window, meta_ready)
+
+
+def attn_decode_rope_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv, hd, scale,
+                               n_splits=None, err=None, window=0, meta_ready=False):
+    """`attn_decode_quantized` with the rotation and the append fused in: `qkv` holds the raw projections of one new token per sequence;
+    the rotated keys and the values are written into the cache as codes, the same as `rope_quantize_append` writes."""
+    _need(cos is not None and sin is not None, "attn_decode_rope_quantized: needs the position table")
+    _attn_decode_quantized("attn_decode_rope_quantized", qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv,
+                           hd, scale, n_splits, err, window, meta_ready)
