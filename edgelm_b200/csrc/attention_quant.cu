@@ -1,9 +1,12 @@
 // Entry points of the attention over the 8-bit cache.
 #include "attention_quant_decode.cuh"
+#include "attention_quant_prefill.cuh"
 
 namespace edgelm {
 int launch_decode_quant_int8(const QuantDecodeArgs& p, int dtype, int hd, int n_seqs, int n_splits, int warps, cudaStream_t stream);
 int launch_decode_quant_fp8(const QuantDecodeArgs& p, int dtype, int hd, int n_seqs, int n_splits, int warps, cudaStream_t stream);
+int launch_prefill_quant_int8(const QuantPrefillArgs& p, int dtype, int hd, int n_tiles, int n_splits, cudaStream_t stream);
+int launch_prefill_quant_fp8(const QuantPrefillArgs& p, int dtype, int hd, int n_tiles, int n_splits, cudaStream_t stream);
 }  // namespace edgelm
 
 using namespace edgelm;
@@ -37,6 +40,35 @@ extern "C" int edgelm_attn_decode_quantized(const void* q, long long ldq, void* 
   const int warps = (long long)n_seqs * nkv * chunks * n_splits <= 148 ? 8 : 4;
   const int rc = format == QF_INT8 ? launch_decode_quant_int8(p, dtype, hd, n_seqs, n_splits, warps, stream)
                                    : launch_decode_quant_fp8(p, dtype, hd, n_seqs, n_splits, warps, stream);
+  if (rc) return rc;
+  EL_LAUNCH_CHECK(who);
+  return 0;
+}
+
+// New tokens, any number a sequence, as tiles of at most `max_tile_tokens` (up to 128) consecutive tokens of one sequence; their keys and
+// values are in the cache already.  n_splits: blocks that share a row tile's keys, 1 to 8.
+extern "C" int edgelm_attn_prefill_quantized(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache,
+                                             const float* k_scale, const float* v_scale, int dtype, int format, const int32_t* page_table,
+                                             int table_stride, int n_pages, const int32_t* seq_slot, const int32_t* tile_seq, const int32_t* tile_tok0,
+                                             const int32_t* tile_ntok, const int32_t* tile_pos0, int n_tiles, int max_tile_tokens, int nh, int nkv,
+                                             int hd, float scale, int n_splits, int window, int* err, cudaStream_t stream) {
+  if (n_tiles == 0) return 0;
+  const char* who = "attn_prefill_quantized";
+  EL_REFUSE(nh > 0 && nkv > 0 && nh % nkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, nh, nkv);
+  EL_REFUSE(hd >= 16 && hd <= 256 && hd % 16 == 0, "%s: head size %d (takes 16..256 in steps of 16)", who, hd);
+  EL_REFUSE((format == QF_INT8 || format == QF_FP8) && (dtype == DT_F32 || dtype == DT_BF16), "%s: format %d, dtype %d", who, format, dtype);
+  EL_REFUSE(n_tiles > 0 && max_tile_tokens >= 1 && max_tile_tokens <= 128, "%s: %d tiles of up to %d tokens (takes 1 to 128)", who, n_tiles, max_tile_tokens);
+  EL_REFUSE(n_splits >= 1 && n_splits <= QP_MAX_SPLITS, "%s: %d splits (takes 1 to %d)", who, n_splits, QP_MAX_SPLITS);
+  EL_REFUSE(window >= 0 && n_pages > 0, "%s: a window of %d keys, %d pages", who, window, n_pages);
+  EL_REFUSE((uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0 && (uintptr_t)k_scale % 16 == 0 && (uintptr_t)v_scale % 16 == 0,
+            "%s: the cache must start on 16-byte boundaries", who);
+  EL_REFUSE((uintptr_t)q % 16 == 0 && ldq % 4 == 0, "%s: query rows must start on a 16-byte boundary, a multiple of 4 numbers apart", who);
+  EL_REFUSE((uintptr_t)out % 8 == 0 && ldo % 2 == 0, "%s: output rows must start on 8-byte boundaries", who);
+  const int per_tile = (max_tile_tokens * (nh / nkv) + QP_ROWS - 1) / QP_ROWS;
+  EL_REFUSE(nkv <= 65535 && (long long)n_tiles * per_tile <= 65535, "%s: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", who, n_tiles, per_tile);
+  const QuantPrefillArgs p = {q, out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok,
+                              tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, scale};
+  const int rc = format == QF_INT8 ? launch_prefill_quant_int8(p, dtype, hd, n_tiles, n_splits, stream) : launch_prefill_quant_fp8(p, dtype, hd, n_tiles, n_splits, stream);
   if (rc) return rc;
   EL_LAUNCH_CHECK(who);
   return 0;

@@ -1,14 +1,15 @@
 // What the attention kernels over the 8-bit cache share: float16 products of codes, and the arithmetic of scores and weights.
 //
 // With codes a (keys) and c (values) and scales u_j, v_j:   out = sum_j p_j v_j c_j / sum_j p_j,   p_j = 2^(s_j - m),
-// s_j = log2(e) scale u_j (q . a_j).  Let v_j = f_j 2^e_j, e_j the float's exponent (held to -40 at least).  The kernels keep
-//     x_j = s_j + e_j,   t_j = 2^(x_j - M + 60),   M >= x_j for all j so far,
-// and sum   w_j c_j  with w_j = t_j f_j 2^-46 (the operand of the product with the codes: a float16 number under 2^15), and t_j 2^-e_j
+// s_j = log2(e) scale u_j (q . a_j).  Let v_j = f_j 2^e_j, e_j the float's exponent (held to -60 at least).  The kernels keep
+//     x_j = s_j + e_j,   t_j = 2^(x_j - M + 46),   M >= x_j for all j so far,
+// and sum   w_j c_j  with w_j = t_j f_j 2^-32 (the operand of the product with the codes: a float16 number under 2^15), and t_j 2^-e_j
 // (the same weight without its value's scale, in float32).  A weight is small beside the largest *weighted* row only, whatever the
 // scales of the rows, so no scale pushes the operand out of float16's range: 2^14 keeps 28 bits below the largest weight above
-// float16's smallest number, and rows that are all under 2^-33 have at least 11 (f down to 2^-27).  2^60 is as far from float32's
-// largest number (2^100 a row, with e = -40) as rows that weigh nothing in the sum of values, but count in the other, are from its
-// smallest.  Taking e_j off the float is exact and costs no logarithm.
+// float16's smallest normal number (a key is off by 2^-39 of the largest weighted row at most, besides its operand's rounding), and where all rows' scales lie under 2^-60 (the format's smallest is 2^-67 or so) 11 bits are left down to
+// 2^-87.  2^46 holds the other sum apart from both ends of float32: a term is at most 2^106, and rows drop out of it only where their
+// scale lies 150 powers of two or more under that of a row they compete with.  Taking e_j off the float is exact and costs no
+// logarithm.
 //
 // The queries' rows are brought to at most 2^13 by a power of two before they become float16 numbers (28 bits below a row's largest
 // number survive); float32 models carry a second term, x - float16(x), of queries and weights: 22 bits.
@@ -17,9 +18,9 @@
 
 namespace edgelm {
 
-constexpr float AQ_LIFT = 60.f;            // t <= 2^60
-constexpr float AQ_OPERAND = 1.4210854715202004e-14f;   // 2^-46: the largest weight as an operand is 2^14 to 2^15
-constexpr float AQ_OPERAND_BACK = 70368744177664.f;     // 2^46, for the finished sums of values
+constexpr float AQ_LIFT = 46.f;            // t <= 2^46
+constexpr float AQ_OPERAND = 2.3283064365386963e-10f;   // 2^-32: the largest weight as an operand is 2^14 to 2^15
+constexpr float AQ_OPERAND_BACK = 4294967296.f;         // 2^32, for the finished sums of values
 constexpr int AQ_QUERY_EXP = 12;           // a query row's largest number lies in [2^12, 2^13)
 constexpr float AQ_LOG2E = 1.4426950408889634f;
 constexpr long long AQ_WAIT_CYCLES = 2000000000LL;
@@ -51,12 +52,12 @@ __device__ __forceinline__ uint32_t aq_transpose8(uint32_t x) {   // an 8 x 8 ma
   return y;
 }
 
-// A value's scale as f 2^e, f with the operand's 2^-46 (f keeps a NaN).
+// A value's scale as f 2^e, f with the operand's 2^-32 (f keeps a NaN).
 struct ValueScale {
   float e, f, undo;    // undo = 2^-e
 };
 __device__ __forceinline__ ValueScale value_scale(float v) {
-  const int b = min(max((int)((__float_as_uint(v) >> 23) & 255u), 127 - 40), 253);
+  const int b = min(max((int)((__float_as_uint(v) >> 23) & 255u), 127 - 60), 253);
   const float undo = __uint_as_float((uint32_t)(254 - b) << 23);
   return {(float)(b - 127), v * undo * AQ_OPERAND, undo};
 }

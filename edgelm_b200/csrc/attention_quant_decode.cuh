@@ -19,6 +19,7 @@ namespace edgelm {
 
 constexpr int QD_HEADS = 8;        // query heads of a block
 constexpr int QD_STAGES = 2;
+constexpr int QD_MAX_WARPS = 8;
 constexpr int QD_MAX_SPLITS = 16;  // blocks of a cluster
 
 __host__ __device__ constexpr int qd_tile_keys(int hdt) { return hdt <= 4 ? 64 : hdt <= 8 ? 32 : 16; }   // about 8 KB of codes

@@ -1,33 +1,41 @@
-// Host side of the decode attention over the 8-bit cache: one instantiation a head size, format and type (a source file a format).
+// Host side of the attention over the 8-bit cache: one instantiation a head size, format and type (a source file a kernel and format).
 #pragma once
+#include <atomic>
 #include <utility>
 
 #include "attention_quant_decode.cuh"
+#include "attention_quant_prefill.cuh"
 
 namespace edgelm {
 
-template <int FMT, typename T, int HDT>
-static cudaError_t launch_decode_quant_one(const QuantDecodeArgs& p, int n_seqs, int n_splits, int warps, cudaStream_t stream) {
-  auto kern = attn_decode_quant_kernel<HDT, FMT, T>;
-  const int smem = qd_smem(HDT, sizeof(T) == 4 ? 2 : 1, warps);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && n_splits > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e != cudaSuccess) return e;
-  const int chunks = (p.nh / p.nkv + QD_HEADS - 1) / QD_HEADS;
+// What a kernel needs once a device (a bit a device): shared memory, and clusters of more than 8 blocks.
+template <typename K>
+static cudaError_t quant_kernel_ready(K kern, int smem, bool wide_clusters, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && done.load(std::memory_order_acquire) >> dev & 1)) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return e;
+}
+
+template <typename K, typename A>
+static cudaError_t launch_quant_kernel(K kern, dim3 grid, int threads, int smem, int pdl_bit, const A& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n_splits, p.nkv * chunks, n_seqs);
-  cfg.blockDim = dim3(warps * 32);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (n_splits > 1) {
+  if (grid.x > 1) {      // the blocks that share keys: a cluster
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = n_splits;
+    attr[n].val.clusterDim.x = grid.x;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (pdl_enabled() & 2) {
+  if (pdl_enabled() & pdl_bit) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
@@ -35,6 +43,27 @@ static cudaError_t launch_decode_quant_one(const QuantDecodeArgs& p, int n_seqs,
   cfg.attrs = attr;
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+template <int FMT, typename T, int HDT>
+static cudaError_t launch_decode_quant_one(const QuantDecodeArgs& p, int n_seqs, int n_splits, int warps, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+  auto kern = attn_decode_quant_kernel<HDT, FMT, T>;
+  const cudaError_t e = quant_kernel_ready(kern, qd_smem(HDT, TERMS, QD_MAX_WARPS), true, done);
+  if (e != cudaSuccess) return e;
+  const int chunks = (p.nh / p.nkv + QD_HEADS - 1) / QD_HEADS;
+  return launch_quant_kernel(kern, dim3(n_splits, p.nkv * chunks, n_seqs), warps * 32, qd_smem(HDT, TERMS, warps), 2, p, stream);
+}
+
+template <int FMT, typename T, int HDT>
+static cudaError_t launch_prefill_quant_one(const QuantPrefillArgs& p, int n_tiles, int n_splits, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+  auto kern = attn_prefill_quant_kernel<HDT, FMT, T>;
+  const cudaError_t e = quant_kernel_ready(kern, qp_smem(HDT, TERMS), false, done);
+  if (e != cudaSuccess) return e;
+  return launch_quant_kernel(kern, dim3(n_splits, p.nkv, n_tiles * p.blocks_per_tile), QP_THREADS, qp_smem(HDT, TERMS), 16, p, stream);
 }
 
 template <int FMT, typename T, int... I>
@@ -52,6 +81,25 @@ static int launch_decode_quant(const QuantDecodeArgs& p, int dtype, int hd, int 
                                         : launch_decode_quant_sizes<FMT, __nv_bfloat16>(sizes, p, hd, n_seqs, n_splits, warps, stream);
   if (e != cudaSuccess) {
     set_error("attn_decode_quantized: launch failed: %s", cudaGetErrorString(e));
+    return -2;
+  }
+  return 0;
+}
+
+template <int FMT, typename T, int... I>
+static cudaError_t launch_prefill_quant_sizes(std::integer_sequence<int, I...>, const QuantPrefillArgs& p, int hd, int n_tiles, int n_splits, cudaStream_t stream) {
+  cudaError_t e = cudaErrorInvalidValue;
+  ((hd == 16 * (I + 1) ? (void)(e = launch_prefill_quant_one<FMT, T, I + 1>(p, n_tiles, n_splits, stream)) : (void)0), ...);
+  return e;
+}
+
+template <int FMT>
+static int launch_prefill_quant(const QuantPrefillArgs& p, int dtype, int hd, int n_tiles, int n_splits, cudaStream_t stream) {
+  const auto sizes = std::make_integer_sequence<int, 16>{};
+  const cudaError_t e = dtype == DT_F32 ? launch_prefill_quant_sizes<FMT, float>(sizes, p, hd, n_tiles, n_splits, stream)
+                                        : launch_prefill_quant_sizes<FMT, __nv_bfloat16>(sizes, p, hd, n_tiles, n_splits, stream);
+  if (e != cudaSuccess) {
+    set_error("attn_prefill_quantized: launch failed: %s", cudaGetErrorString(e));
     return -2;
   }
   return 0;

@@ -1560,36 +1560,57 @@ def _entry(name, kinds):
     return fn
 
 
-def _a(t):
-    return t.data_ptr() if t is not None else None
-
-
 def _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what):
-    """Checks the cache's tensors; the format's code."""
+    """Checks the cache's tensors; the format's code and the device's index.  (Messages are made only when something is wrong: these
+    calls are made once a layer and token.)"""
     code = _QUANT_CODES.get(kcache.dtype)
-    _need(code is not None and vcache.dtype == kcache.dtype, f"{what}: the cache's codes must be int8 or float8_e4m3fn, keys and values alike")
+    if code is None or vcache.dtype != kcache.dtype:
+        raise KernelError(f"{what}: the cache's codes must be int8 or float8_e4m3fn, keys and values alike")
     shape = kcache.shape
-    _need(len(shape) == 4 and shape[1:] == (nkv, PAGE, hd) and vcache.shape == shape, f"{what}: codes must be [pages, {nkv}, {PAGE}, {hd}]")
-    _need(k_scale.shape == shape[:3] and v_scale.shape == shape[:3] and k_scale.dtype == v_scale.dtype == torch.float32, f"{what}: scales must be float32 [pages, {nkv}, {PAGE}]")
-    _need(kcache.is_contiguous() and vcache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous(), f"{what}: the cache must be contiguous")
-    _need(kcache.is_cuda and kcache.device.index == torch.cuda.current_device(), f"{what}: the cache must lie on the current device")
-    return code
+    if len(shape) != 4 or shape[1:] != (nkv, PAGE, hd) or vcache.shape != shape:
+        raise KernelError(f"{what}: codes must be [pages, {nkv}, {PAGE}, {hd}]")
+    rows = shape[:3]
+    if k_scale.shape != rows or v_scale.shape != rows or not k_scale.dtype == v_scale.dtype == torch.float32:
+        raise KernelError(f"{what}: scales must be float32 [pages, {nkv}, {PAGE}]")
+    if not (kcache.is_contiguous() and vcache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise KernelError(f"{what}: the cache must be contiguous")
+    device = kcache.get_device()
+    if device < 0 or device != torch.cuda.current_device() or not device == vcache.get_device() == k_scale.get_device() == v_scale.get_device():
+        raise KernelError(f"{what}: the cache must lie on the current device")
+    return code, device
 
 
-def _quant_steps(page_table, tensors, what):
-    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_cuda and page_table.stride(1) == 1, f"{what}: the page table must be int32 rows")
-    for t, name in tensors:
-        _need(t.dtype == torch.int32 and t.is_cuda and t.is_contiguous(), f"{what}: {name} must be a contiguous int32 CUDA tensor")
+def _quant_steps(page_table, tensors, device, what):
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.get_device() != device or page_table.stride(1) != 1:
+        raise KernelError(f"{what}: the page table must be int32 rows on the cache's device")
+    for t, n in tensors:
+        if t.dtype != torch.int32 or t.get_device() != device or not t.is_contiguous() or t.numel() < n:
+            raise KernelError(f"{what}: positions, indices, tiles and the error word must be contiguous int32 tensors on the cache's device, one number each "
+                              f"per token, sequence or tile (at least {n} here)")
 
 
-def _quant_tables(cos, sin, hd, what):
-    _need(cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd // 2 and
-          cos.is_contiguous() and sin.is_contiguous() and cos.is_cuda and sin.is_cuda, f"{what}: table layout")
+def _quant_tables(cos, sin, hd, device, what):
+    if not (cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd // 2 and
+            cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == device):
+        raise KernelError(f"{what}: the position tables must be float32 [positions, {hd // 2}] on the cache's device")
 
 
 def _heads(nh, nkv, hd, what):
-    _need(nh > 0 and nkv > 0 and nh % nkv == 0, f"{what}: {nh} query heads are not a multiple of {nkv} key/value heads")
-    _need(16 <= hd <= 256 and hd % 16 == 0, f"{what}: head size {hd} (takes 16 to 256 in steps of 16)")
+    if nh <= 0 or nkv <= 0 or nh % nkv:
+        raise KernelError(f"{what}: {nh} query heads are not a multiple of {nkv} key/value heads")
+    if not 16 <= hd <= 256 or hd % 16:
+        raise KernelError(f"{what}: head size {hd} (takes 16 to 256 in steps of 16)")
+
+
+def _quant_rows(q, out, width, nh, hd, device, what):
+    if q.dtype != out.dtype or q.dim() != 2 or out.dim() != 2 or q.stride(1) != 1 or out.stride(1) != 1:
+        raise KernelError(f"{what}: queries and outputs must be rows of one type")
+    if q.shape[1] < width or out.shape[1] < nh * hd or q.get_device() != device or out.get_device() != device:
+        raise KernelError(f"{what}: rows of {width} and {nh * hd} numbers on the cache's device are wanted")
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, kcache, vcache, k_scale, v_scale, nh, nkv, hd, err):
@@ -1597,31 +1618,34 @@ def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, 
     as codes and scales into their pages."""
     what = "rope_quantize_append"
     _heads(nh, nkv, hd, what)
+    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    if not qkv.is_contiguous() or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd or qkv.get_device() != device:
+        raise KernelError(f"{what}: the projections must be contiguous rows of {(nh + 2 * nkv) * hd} numbers on the cache's device")
     T = qkv.shape[0]
-    _need(qkv.is_contiguous() and qkv.dim() == 2 and qkv.shape[1] == (nh + 2 * nkv) * hd, f"{what}: qkv layout")
-    code = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
-    _quant_tables(cos, sin, hd, what)
-    _quant_steps(page_table, ((tok_pos, "tok_pos"), (tok_seq, "tok_seq"), (seq_slot, "seq_slot"), (err, "err")), what)
-    _need(tok_pos.numel() >= T and tok_seq.numel() >= T, f"{what}: one position and one sequence index per token")
+    _quant_tables(cos, sin, hd, device, what)
+    _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
     _check(_entry("edgelm_rope_quantize_append", "piipppp" "iippi" "pppp" "iiiipp")(
-        _a(qkv), _dt(qkv), code, _a(tok_pos), _a(tok_seq), _a(seq_slot), _a(page_table), page_table.stride(0), kcache.shape[0], _a(cos), _a(sin),
-        cos.shape[0], _a(kcache), _a(vcache), _a(k_scale), _a(v_scale), T, nh, nkv, hd, _a(err), torch.cuda.current_stream().cuda_stream),
-        launches=1 if T else 0)
+        qkv.data_ptr(), _dt(qkv), code, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+        kcache.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        T, nh, nkv, hd, err.data_ptr(), _raw_stream(device)), launches=1 if T else 0)
 
 
 def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot, page_table, keys, values, err):
     """keys[t], values[t] = what the 8-bit cache holds for token t (position tok_pos[t] of sequence tok_seq[t]): [T, kv_heads, head_dim],
     float32 or bfloat16, code * scale in float32 rounded once.  A token whose page the cache does not have: zeros, and a bit of `err`."""
     what = "quantized_rows"
-    _need(keys.dim() == 3 and keys.shape == values.shape and keys.dtype == values.dtype and keys.is_contiguous() and values.is_contiguous() and keys.is_cuda, f"{what}: rows must be contiguous [tokens, kv_heads, head_dim]")
+    if keys.dim() != 3 or keys.shape != values.shape or keys.dtype != values.dtype or not (keys.is_contiguous() and values.is_contiguous()):
+        raise KernelError(f"{what}: rows must be contiguous [tokens, kv_heads, head_dim], keys and values alike")
     T, nkv, hd = keys.shape
     _heads(nkv, nkv, hd, what)
-    code = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
-    _quant_steps(page_table, ((tok_pos, "tok_pos"), (tok_seq, "tok_seq"), (seq_slot, "seq_slot"), (err, "err")), what)
-    _need(tok_pos.numel() >= T and tok_seq.numel() >= T, f"{what}: one position and one sequence index per token")
+    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    if not keys.get_device() == values.get_device() == device:
+        raise KernelError(f"{what}: rows must lie on the cache's device")
+    _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
     _check(_entry("edgelm_quantized_rows", "ppppi" "ppppii" "ppi" "iiipp")(
-        _a(kcache), _a(vcache), _a(k_scale), _a(v_scale), code, _a(tok_pos), _a(tok_seq), _a(seq_slot), _a(page_table), page_table.stride(0),
-        kcache.shape[0], _a(keys), _a(values), _dt(keys), T, nkv, hd, _a(err), torch.cuda.current_stream().cuda_stream), launches=1 if T else 0)
+        kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), code, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(),
+        page_table.data_ptr(), page_table.stride(0), kcache.shape[0], keys.data_ptr(), values.data_ptr(), _dt(keys), T, nkv, hd, err.data_ptr(),
+        _raw_stream(device)), launches=1 if T else 0)
 
 
 def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
@@ -1638,24 +1662,24 @@ def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
 def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv, hd, scale, n_splits,
                            err, window, meta_ready):
     _heads(nh, nkv, hd, what)
-    _need(q.dtype == out.dtype and q.dim() == 2 and out.dim() == 2 and q.stride(1) == 1 and out.stride(1) == 1, f"{what}: rows must be contiguous, of one type")
-    width = nh * hd if cos is None else (nh + 2 * nkv) * hd
-    _need(q.shape[0] >= n_seqs and out.shape[0] >= n_seqs and q.shape[1] >= width and out.shape[1] >= nh * hd and out.is_cuda and q.is_cuda, f"{what}: shapes")
-    code = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
-    _quant_steps(page_table, ((seq_slot, "seq_slot"), (seq_pos, "seq_pos")) + (((err, "err"),) if err is not None else ()), what)
-    _need(seq_slot.numel() >= n_seqs and seq_pos.numel() >= n_seqs, f"{what}: one slot and one position per sequence")
+    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    _quant_rows(q, out, nh * hd if cos is None else (nh + 2 * nkv) * hd, nh, hd, device, what)
+    if n_seqs < 0 or q.shape[0] < n_seqs or out.shape[0] < n_seqs:
+        raise KernelError(f"{what}: a row of queries and of outputs per sequence is wanted")
+    _quant_steps(page_table, ((seq_slot, n_seqs), (seq_pos, n_seqs)) + (((err, 1),) if err is not None else ()), device, what)
     window = int(window or 0)
     if n_splits is None:
         keys = page_table.shape[1] * PAGE
-        n_splits = quantized_decode_splits(n_seqs, nh, nkv, hd, min(keys, window) if window else keys)
+        n_splits = quantized_decode_splits(n_seqs, nh, nkv, hd, min(keys, window) if window > 0 else keys)
+    cos_ptr = sin_ptr = None
     max_pos = 0
     if cos is not None:
-        _quant_tables(cos, sin, hd, what)
-        max_pos = cos.shape[0]
+        _quant_tables(cos, sin, hd, device, what)
+        cos_ptr, sin_ptr, max_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
     _check(_entry("edgelm_attn_decode_quantized", "plplpppp" "iipiipp" "ppi" "iiiif" "iiipp")(
-        _a(q), q.stride(0), _a(out), out.stride(0), _a(kcache), _a(vcache), _a(k_scale), _a(v_scale), _dt(q), code, _a(page_table),
-        page_table.stride(0), kcache.shape[0], _a(seq_slot), _a(seq_pos), _a(cos), _a(sin), max_pos, n_seqs, nh, nkv, hd, scale, n_splits, window,
-        1 if meta_ready else 0, _a(err), torch.cuda.current_stream().cuda_stream), launches=1 if n_seqs else 0)
+        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _dt(q), code,
+        page_table.data_ptr(), page_table.stride(0), kcache.shape[0], seq_slot.data_ptr(), seq_pos.data_ptr(), cos_ptr, sin_ptr, max_pos, n_seqs, nh, nkv,
+        hd, scale, n_splits, window, 1 if meta_ready else 0, err.data_ptr() if err is not None else None, _raw_stream(device)), launches=1 if n_seqs else 0)
 
 
 def attn_decode_quantized(q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, n_seqs, nh, nkv, hd, scale, n_splits=None,
@@ -1675,3 +1699,37 @@ def attn_decode_rope_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_
     _need(cos is not None and sin is not None, "attn_decode_rope_quantized: needs the position table")
     _attn_decode_quantized("attn_decode_rope_quantized", qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv,
                            hd, scale, n_splits, err, window, meta_ready)
+
+
+def quantized_prefill_splits(n_blocks, hd, max_keys, n_sms=148):
+    """Blocks that share a row tile's keys in the prompt attention over the 8-bit cache, given how many there would be without."""
+    tile = 64 if hd <= 128 else 32
+    splits = 1
+    while splits < 8 and n_blocks * splits < n_sms and 2 * tile * splits < max_keys:
+        splits *= 2
+    return splits
+
+
+def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok, tile_pos0, n_tiles, nh, nkv,
+                           hd, scale, err=None, window=0, max_keys=0, n_splits=None):
+    """`attn_prefill` over the 8-bit cache: causal attention of new tokens (any number per sequence), as tiles of at most
+    QUANT_PREFILL_TILE consecutive tokens of one sequence; the tokens' own keys and values are in the cache.  `max_keys`: the longest
+    sequence's keys, if the caller knows them (0: the page table's width), by which the blocks that share keys are counted."""
+    what = "attn_prefill_quantized"
+    _heads(nh, nkv, hd, what)
+    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    _quant_rows(qkv, out, nh * hd, nh, hd, device, what)
+    if qkv.shape[0] != out.shape[0]:
+        raise KernelError(f"{what}: a row of outputs per row of queries is wanted")
+    _quant_steps(page_table, ((seq_slot, 0), (tile_seq, n_tiles), (tile_tok0, n_tiles), (tile_ntok, n_tiles), (tile_pos0, n_tiles)) +
+                 (((err, 1),) if err is not None else ()), device, what)
+    window = int(window or 0)
+    most = max(1, min(QUANT_PREFILL_TILE, qkv.shape[0]))
+    if n_splits is None:
+        keys = max_keys or page_table.shape[1] * PAGE
+        n_splits = quantized_prefill_splits(nkv * n_tiles * -(-most * (nh // nkv) // 64), hd, min(keys, window + most) if window > 0 else keys)
+    _check(_entry("edgelm_attn_prefill_quantized", "plplpppp" "iipii" "ppppp" "iiiii" "fiipp")(
+        qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _dt(qkv),
+        code, page_table.data_ptr(), page_table.stride(0), kcache.shape[0], seq_slot.data_ptr(), tile_seq.data_ptr(), tile_tok0.data_ptr(),
+        tile_ntok.data_ptr(), tile_pos0.data_ptr(), n_tiles, most, nh, nkv, hd, scale, n_splits, window, err.data_ptr() if err is not None else None,
+        _raw_stream(device)), launches=1 if n_tiles else 0)

@@ -54,9 +54,9 @@ def attend(q, first, keys, values, scale, window=0):
     if window:
         seen &= j > p - window
     w = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
-    w = torch.where(seen, w, torch.zeros_like(w))
-    v = torch.where(seen.any(0)[:, None, None], v, torch.zeros_like(v))
-    return torch.einsum("hnl,lhd->nhd", w, v)
+    out = torch.einsum("hnl,lhd->nhd", w, v.nan_to_num(0.0, math.inf, -math.inf))
+    reached = torch.einsum("nl,lhd->nhd", seen.double(), torch.isnan(v).double()) > 0      # a value that is no number, seen
+    return out.masked_fill(reached, math.nan)
 
 
 def tables(n, hd, device, theta=10000.0):

@@ -34,7 +34,9 @@ def off_bound(q, first, keys, values, scale, window, exact, dtype, given_bf16):
     d = u_q sum |q_i k_i| scale, and every weight by a factor within 1 +- 2 d (numerator and denominator), the weights' own rounding
     by u_w, and the output is rounded once.  float16 terms: u = 2^-11 of one, 2^-22 of two (a bfloat16 query row is exact down to
     2^-14 of its largest number once lifted, taken as 2^-11 all the same); scores and exponents themselves are float32 sums: 2^-20 of
-    the sum of their terms' magnitudes, the value's exponent of up to 2^5 and the reference among them."""
+    the sum of their terms' magnitudes, the value's exponent of up to 2^5 and the reference among them.  Weighted rows far below the
+    largest: a weight as operand is at most half of float16's smallest step (2^-25) off, and the largest one is 2^14 at least, so every
+    key adds up to 2^-39 of the largest weighted row's largest number (matters where that row's own number is zero)."""
     n, nh, hd = q.shape
     g = nh // keys.shape[1]
     size = torch.einsum("nhd,lhd->hnl", q.abs(), keys.abs().repeat_interleave(g, 1)) * scale
@@ -43,7 +45,8 @@ def off_bound(q, first, keys, values, scale, window, exact, dtype, given_bf16):
     d = u * size.nan_to_num(0.0)[..., :last].amax(-1) + 2.0 ** -20 * (size.nan_to_num(0.0)[..., :last].amax(-1) + 32.0)      # [nh, n]
     a = ref.attend(q, first, keys, values.abs(), scale, window)
     half_ulp = torch.finfo(dtype).eps / 2
-    return exact.abs() * half_ulp + a * (2 * d.T[..., None] + 2 * u + 2.0 ** -20)
+    floor = 2.0 ** -39 * last * ref.attend(q, first, keys, values.abs().amax(-1, keepdim=True), scale, window)
+    return floor + exact.abs() * half_ulp + a * (2 * d.T[..., None] + 2 * u + 2.0 ** -20)
 
 
 def check(out, exact, bound):

@@ -1,0 +1,146 @@
+"""Prompt attention over the 8-bit cache against its plain statement (tests/quant_reference.py)."""
+import math
+
+import pytest
+import torch
+
+from edgelm_b200.csrc import ops
+from tests import quant_reference as ref
+from tests.test_quant_cache_gpu import DEV, DTYPES, cache_args, check, i32, off_bound, same, word
+
+pytestmark = pytest.mark.gpu
+
+
+def tiles_of(totals, news, size=128):
+    rows, t0 = [], 0
+    for b, (n, m) in enumerate(zip(totals, news)):
+        rows += [(b, t0 + a, min(size, m - a), n - m + a) for a in range(0, m, size)]
+        t0 += m
+    return [i32(r[i] for r in rows) for i in range(4)], len(rows)
+
+
+def prompt_case(fmt, dtype, nh, nkv, hd, totals, news, window=0, splits=None, seed=1, spoil=True, change=None, size=128, max_keys=0, pad=0):
+    dtype = DTYPES[dtype]
+    cache, table = ref.make_cache(fmt, nkv, hd, totals, DEV, seed, k_size=1.5)
+    if spoil:     # what lies behind a sequence's end is not its own: no number at all
+        for b, n in enumerate(totals):
+            if n % 64:
+                p = int(table[b, n // 64])
+                cache["ks"][p, :, n % 64:] = float("nan")
+                cache["vs"][p, :, n % 64:] = float("inf")
+                if fmt == "fp8":
+                    cache["v"].view(torch.int8)[p, :, n % 64:] = 0x7f
+                    cache["k"].view(torch.int8)[p, :, n % 64:] = 0x7f
+    if change:
+        change(cache, table)
+    before = {k: v.clone() for k, v in cache.items()}
+    T = sum(news)
+    q = torch.randn((T, (nh + 2 * nkv) * hd + pad), generator=torch.Generator().manual_seed(seed + 1)).to(dtype).to(DEV)
+    out = torch.full((T, nh * hd + 16), 3.0, dtype=dtype, device=DEV)
+    err, scale = word(), 1 / math.sqrt(hd)
+    tiles, n_tiles = tiles_of(totals, news, size)
+    ops.attn_prefill_quantized(q, out[:, :nh * hd], *cache_args(cache), table, i32(range(len(totals))), *tiles, n_tiles, nh, nkv, hd, scale, err=err, window=window,
+                               max_keys=max_keys, n_splits=splits)
+    assert int(err) == 0 and bool((out[:, nh * hd:] == 3.0).all())
+    for k in before:
+        assert same(before[k], cache[k])
+    t0 = 0
+    for b, (n, m) in enumerate(zip(totals, news)):
+        keys, values = ref.sequence_rows(cache, table[b], n)
+        qq = q[t0:t0 + m, :nh * hd].double().view(m, nh, hd)
+        exact = ref.attend(qq, n - m, keys, values, scale, window)
+        check(out[t0:t0 + m, :nh * hd].view(m, nh, hd), exact, off_bound(qq, n - m, keys, values, scale, window, exact, dtype, True))
+        t0 += m
+    return out[:, :nh * hd].view(T, nh, hd)
+
+
+TOTALS, NEWS = [1, 17, 64, 65, 200, 400, 300], [1, 17, 64, 2, 200, 129, 1]
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 4, 64), (4, 1, 128), (3, 3, 32), (6, 2, 96), (2, 1, 16), (5, 1, 48), (3, 1, 80), (2, 2, 256), (12, 1, 64),
+                                       (24, 2, 112), (7, 1, 192), (2, 1, 208), (2, 2, 144)])
+def test_prompt_heads_and_lengths(fmt, dtype, nh, nkv, hd):
+    prompt_case(fmt, dtype, nh, nkv, hd, TOTALS, NEWS)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 8])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 1, 128), (3, 1, 256)])
+def test_prompt_splits(splits, dtype, nh, nkv, hd):
+    prompt_case("int8", dtype, nh, nkv, hd, TOTALS + [2500], NEWS + [70], splits=splits)
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 130, 5000])
+def test_prompt_window(window):
+    prompt_case("int8", "bf16", 9, 3, 64, TOTALS, NEWS, window=window)
+    prompt_case("fp8", "f32", 4, 1, 128, TOTALS, NEWS, window=window, splits=4)
+    prompt_case("fp8", "bf16", 2, 2, 160, TOTALS, NEWS, window=window)
+
+
+def test_prompt_long_and_smaller_tiles():
+    prompt_case("fp8", "bf16", 4, 2, 64, [1500], [1500])
+    prompt_case("int8", "bf16", 4, 4, 64, [64 * 40 + 3], [300], splits=1)     # more tiles of keys than a lane of the copying warp holds pages of
+    for size in (1, 5, 64, 100):
+        prompt_case("int8", "bf16", 6, 2, 64, [130, 70], [130, 33], size=size, max_keys=130)
+
+
+def test_prompt_rows_lie_where_the_strides_say():
+    prompt_case("int8", "bf16", 9, 3, 64, TOTALS, NEWS, pad=24)
+    prompt_case("fp8", "f32", 9, 3, 48, TOTALS, NEWS, pad=4)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prompt_scales_of_all_sizes(fmt, dtype):
+    def change(cache, table):
+        cache["vs"].mul_((10.0 ** (torch.rand(cache["vs"].shape, generator=torch.Generator().manual_seed(9)) * 40 - 20)).to(DEV))
+        cache["v"].view(torch.int8)[:, :, ::7] = 0
+        cache["vs"][:, :, ::7] = 2.0 ** -60 / ref.TOP[fmt]
+    prompt_case(fmt, dtype, 9, 3, 64, [200, 70], [200, 7], change=change, spoil=False)
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+def test_prompt_a_row_that_is_no_number_reaches_who_sees_it(splits):
+    def change(cache, table):
+        cache["vs"][int(table[0, 1]), 0, 5] = float("nan")       # value of position 69, kv head 0
+        cache["v"].view(torch.int8)[int(table[0, 1]), 0, 5] = 0
+        cache["ks"][int(table[0, 0]), 1, 3] = float("nan")       # key of position 3, kv head 1
+        cache["k"].view(torch.int8)[int(table[0, 0]), 1, 3] = 0
+    for window in (0, 50):
+        out = prompt_case("fp8", "bf16", 4, 2, 64, [200], [200], change=change, spoil=False, splits=splits, window=window)
+        nan = torch.isnan(out).all(-1).cpu()
+        p = torch.arange(200)
+        first = (p >= 69) & ((p < 69 + window) if window else p >= 0)
+        second = (p >= 3) & ((p < 3 + window) if window else p >= 0)
+        assert torch.equal(nan, torch.stack([first, first, second, second], 1))
+
+
+def test_prompt_in_a_graph():
+    cache, table = ref.make_cache("int8", 3, 64, [200, 64], DEV, 3)
+    tiles, n = tiles_of([200, 64], [150, 64])
+    q, err = torch.randn((214, 9 * 64), device=DEV).bfloat16(), word()
+    out, captured = torch.empty_like(q), torch.zeros_like(q)
+    run = lambda o: ops.attn_prefill_quantized(q, o, *cache_args(cache), table, i32s, *tiles, n, 9, 3, 64, 0.125, err=err)   # noqa: E731
+    i32s = i32([0, 1])
+    run(out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(captured)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, captured) and int(err) == 0
+    ops.attn_prefill_quantized(q, out, *cache_args(cache), table, i32s, *tiles, 0, 9, 3, 64, 0.125)
+
+
+def test_prompt_pages_that_are_not_there_are_reported():
+    for page in (-1, 99):
+        cache, table = ref.make_cache("int8", 1, 64, [128], DEV, 3)
+        table[0, 0] = page
+        tiles, n = tiles_of([128], [20])
+        err = word()
+        q = torch.randn((20, 128), device=DEV)
+        ops.attn_prefill_quantized(q, torch.empty_like(q), *cache_args(cache), table, i32([0]), *tiles, n, 2, 1, 64, 0.125, err=err)
+        assert int(err) == 4
