@@ -33,28 +33,29 @@ def load_plugins(names=None):
 
 
 def load_engine(model, dtype="bfloat16", ctx=1024, slots=8, max_tokens=None, batch=8192, profile=False, device="cuda:0",
-                use_graphs=True):
+                use_graphs=True, cache_format=None):
     """An Engine for a model folder.  `ctx` is the longest sequence, `slots` how many sequences
     may live at once (together they size the cache, unless `max_tokens` gives its size in
-    tokens directly); `batch` is the most tokens one forward runs (longer steps are cut)."""
+    tokens directly); `batch` is the most tokens one forward runs (longer steps are cut).
+    `cache_format`: None, or "int8" / "fp8" to keep keys and values as 8-bit codes with a scale per row."""
     from .engine.engine import Engine, load_model
     m = load_model(model, dtype, device) if isinstance(model, str) else model
     ctx = min(int(ctx), m.plan.max_positions)
     if max_tokens is None:
         max_tokens = (ctx + 63) // 64 * 64 * int(slots)
-    return Engine(m, max_tokens, max_step_tokens=batch, max_seqs=None, profile=profile, use_graphs=use_graphs)
+    return Engine(m, max_tokens, max_step_tokens=batch, max_seqs=None, profile=profile, use_graphs=use_graphs, cache_format=cache_format)
 
 
 def generate(model, prompts, n=64, temp=0.0, top_k=40, seed=42, stop=None, ignore_eos=False, dtype="bfloat16",
-             ctx=1024, slots=8, engine=None, return_details=False):
+             ctx=1024, slots=8, engine=None, return_details=False, cache_format=None):
     """Generate up to `n` tokens for every prompt (lists of token ids).
 
     `model` is a model folder; or pass a ready `engine`.  Options as edgelm's run command:
     temp (0 = greedy), top_k (40; <= 0 whole vocabulary), seed (42); `stop` defaults to the
     model's eos ids.  Prompts run in batches of at most `slots` sequences, one batch after
-    another.  Returns a list of token lists (or Generation records with return_details)."""
+    another.  `cache_format` as in `load_engine`.  Returns a list of token lists (or Generation records with return_details)."""
     from .engine.generate import GenerationLoop
-    eng = engine or load_engine(model, dtype=dtype, ctx=ctx, slots=slots)
+    eng = engine or load_engine(model, dtype=dtype, ctx=ctx, slots=slots, cache_format=cache_format)
     stop_ids = eng.plan.stop_token_ids if stop is None else stop
     loop = GenerationLoop(eng, SamplingParams(float(temp), int(top_k), int(seed)), max_new_tokens=n, stop_ids=stop_ids,
                           ignore_eos=ignore_eos, max_batch=slots)
@@ -69,8 +70,8 @@ class Session:
     the last position (all positions with all_logits=True); reset() starts over; pos is the
     number of tokens in the cache."""
 
-    def __init__(self, model, dtype="bfloat16", max_ctx=1024, max_batch=128, all_logits=False, profile=False, engine=None):
-        self.engine = engine or load_engine(model, dtype=dtype, ctx=max_ctx, slots=1, batch=max_batch, profile=profile)
+    def __init__(self, model, dtype="bfloat16", max_ctx=1024, max_batch=128, all_logits=False, profile=False, engine=None, cache_format=None):
+        self.engine = engine or load_engine(model, dtype=dtype, ctx=max_ctx, slots=1, batch=max_batch, profile=profile, cache_format=cache_format)
         self.all_logits = all_logits
         self.slot = self.engine.open(1)[0]
 

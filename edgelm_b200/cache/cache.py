@@ -16,6 +16,10 @@ values beside a recurrent state; a block arrangement's own state beside its mixe
 in a NeedSet; each named need joins the group of its kind, and the layer run's entry is a
 `CompositeEntry` that answers `entry[name]`.
 
+With a `format` ("int8" or "fp8") every KV group keeps 8-bit codes and a float32 scale per row of head_dim numbers instead of the
+compute dtype: `entry.k / v` are then the codes, `entry.k_scale / v_scale` [page][kv_head][64] the scales.  Mixers whose kernels
+do not read codes refuse it.  A new page's scales are zero and its codes too: rows of zeros.
+
 Lengths are per slot and shared by all groups.  Everything a step needs on the device about
 the cache (the batch's rows of the page tables) is packed by the engine into the step's
 metadata; this class owns the storage and the bookkeeping.
@@ -27,6 +31,7 @@ from ..parts.base import KVNeed, NeedSet, StateNeed
 from .slots import CacheError, FreeList
 
 PAGE = 64
+FORMATS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 
 
 def pages_for(n_tokens):
@@ -46,6 +51,14 @@ class CacheEntry:
     @property
     def v(self):
         return self.group.v[self.index] if self.group.v is not None else None
+
+    @property
+    def k_scale(self):
+        return self.group.k_scale[self.index]
+
+    @property
+    def v_scale(self):
+        return self.group.v_scale[self.index]
 
     @property
     def state(self):
@@ -80,7 +93,8 @@ class KVGroup:
     whole sequences.  The page table stays indexed by position // 64; entries of pages given back are -1, and the
     attention kernels of a windowed mixer never look before the window."""
 
-    def __init__(self, gid, need, n_entries, n_pages, n_slots, max_pages_per_seq, dtype, device, piece_tokens=None):
+    def __init__(self, gid, need, n_entries, n_pages, n_slots, max_pages_per_seq, dtype, device, piece_tokens=None, format=None):
+        self.format = format                               # None: rows in the compute dtype; else the 8-bit format of the codes
         self.id, self.need, self.n_entries = gid, need, n_entries
         self.window = need.window
         self.pages_per_seq = max_pages_per_seq
@@ -93,13 +107,16 @@ class KVGroup:
         self.n_held = np.zeros(n_slots, dtype=np.int32)
         self.low = np.zeros(n_slots, dtype=np.int32)      # a sequence holds the pages low .. low + n_held - 1
         self.version = 0                                  # counts changes of the table (a step's metadata is patched when it moved)
-        self.k = self.v = self.pooled_k = self.pooled_v = None
+        self.k = self.v = self.pooled_k = self.pooled_v = self.k_scale = self.v_scale = None
         self.v_head_dim = need.v_head_dim or need.head_dim
         self.pool_block = need.pool                        # positions per pooled block (None: no pooled rows)
         if self.pool_block is not None and self.pool_block < 1:
             raise CacheError(f"pooled blocks of {self.pool_block} positions")
         self.pooled_rows = -(-PAGE // self.pool_block) if self.pool_block else 0     # block ends that fall into one page, at most
         if device is not None:
+            dtype = dtype if format is None else FORMATS[format]
+            if format is not None:
+                self.k_scale, self.v_scale = (torch.zeros((n_entries, n_pages, need.n_kv_heads, PAGE), dtype=torch.float32, device=device) for _ in range(2))
             self.k = torch.zeros((n_entries, n_pages, need.n_kv_heads, PAGE, need.head_dim), dtype=dtype, device=device)
             if not need.values_in_keys:
                 self.v = torch.zeros((n_entries, n_pages, need.n_kv_heads, PAGE, self.v_head_dim), dtype=dtype, device=device)
@@ -109,6 +126,8 @@ class KVGroup:
 
     def bytes_per_token(self, itemsize):
         per_row = self.need.head_dim + (0 if self.need.values_in_keys else self.v_head_dim)
+        if self.format is not None:
+            return int(self.n_entries * self.need.n_kv_heads * (per_row + 8))     # a byte a number and a scale for the keys and the values each
         pooled = self.pooled_rows * per_row * 4 / PAGE
         return int(self.n_entries * self.need.n_kv_heads * (per_row * itemsize + pooled))
 
@@ -182,7 +201,10 @@ class SequenceCache:
 
     PIECE_TOKENS = 256   # a sequence of a model with windowed groups brings at most so many tokens to one micro-step
 
-    def __init__(self, needs, max_tokens, max_positions, dtype=torch.float32, device=None, max_seqs=None, piece_tokens=None):
+    def __init__(self, needs, max_tokens, max_positions, dtype=torch.float32, device=None, max_seqs=None, piece_tokens=None, format=None):
+        if format is not None and format not in FORMATS:
+            raise CacheError(f"a cache in the format '{format}'; known: {', '.join(FORMATS)}")
+        self.format = format
         n_pages = pages_for(max_tokens)
         if n_pages <= 0:
             raise CacheError("the cache needs room for at least one page of tokens")
@@ -201,6 +223,11 @@ class SequenceCache:
                     yield from plain(sub)
             elif need is not None:
                 yield need
+        if format is not None:
+            for i, need in enumerate(needs):
+                for kept in plain(need):
+                    if isinstance(kept, KVNeed) and (format not in kept.formats or kept.values_in_keys or kept.pool or kept.v_head_dim not in (None, kept.head_dim)):
+                        raise CacheError(f"schedule entry {i}: its mixer does not read keys and values kept as {format} codes")
         windowed = any(isinstance(n, KVNeed) and n.window is not None for need in needs for n in plain(need))
         # with a windowed group, steps are cut so that a sequence brings at most `piece_tokens` tokens at a time: what
         # such a group must hold per sequence is then the window and one piece, whatever the prompt's length
@@ -222,7 +249,7 @@ class SequenceCache:
             if isinstance(need, KVNeed):
                 if need.window is not None and need.window < 1:
                     raise CacheError(f"a window of {need.window} keys")
-                g = KVGroup(gid, need, len(idxs), n_pages, self.n_slots, self.max_pages_per_seq, dtype, device, self.piece_tokens)
+                g = KVGroup(gid, need, len(idxs), n_pages, self.n_slots, self.max_pages_per_seq, dtype, device, self.piece_tokens, format)
             elif isinstance(need, StateNeed):
                 g = StateGroup(gid, need, len(idxs), self.n_slots, device)
             else:
@@ -349,7 +376,7 @@ class SequenceCache:
         total = 0
         for g in self.groups:
             for t in (getattr(g, "k", None), getattr(g, "v", None), getattr(g, "state", None), getattr(g, "pooled_k", None),
-                      getattr(g, "pooled_v", None)):
+                      getattr(g, "pooled_v", None), getattr(g, "k_scale", None), getattr(g, "v_scale", None)):
                 if t is not None:
                     total += t.numel() * t.element_size()
         return total
@@ -361,6 +388,8 @@ class SequenceCache:
             win = f", the last {g.window} keys of a sequence" if g.window is not None else ""
             if g.pool_block:
                 win += f", a pooled row per {g.pool_block} positions"
+            if g.format is not None:
+                win += f", kept as {g.format} codes with a scale a row"
             lines.append(f"  keys/values of {g.n_entries} layer run(s): {g.need.n_kv_heads} heads of {g.need.head_dim}{win}, {g.n_pages} pages "
                          f"of {PAGE} tokens, {g.bytes_per_token(torch.empty(0, dtype=self.dtype).element_size())} B a token")
         for g in self.state_groups:

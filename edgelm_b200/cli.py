@@ -2,7 +2,7 @@
 run | bench | info | logits with its option names and meanings where it has them.
 
   python -m edgelm_b200 run    -m DIR -p "5,17,3;9,9" [-n 64] [--temp 0.8 --top-k 40 --seed 1] [--dtype bf16|f32]
-                               [--ctx 1024] [--batch 8192] [--slots 8] [--ignore-eos] [--stop 2,7]
+                               [--cache int8|fp8] [--ctx 1024] [--batch 8192] [--slots 8] [--ignore-eos] [--stop 2,7]
                                [--verbose] [--profile trace.json] [--stats]
   python -m edgelm_b200 bench  -m DIR [--prompt-len 128] [--gen 64] [--reps 3] [--batch-sizes 1,8] [--json]
   python -m edgelm_b200 info   -m DIR [--dtype ..] [--ops]
@@ -54,7 +54,7 @@ def _engine(args, model, slots=None, profile=False):
     from .engine.engine import Engine
     ctx = min(args.ctx, model.plan.max_positions)
     slots = slots or args.slots
-    return Engine(model, max_tokens=(ctx + 63) // 64 * 64 * slots, max_step_tokens=args.batch, profile=profile)
+    return Engine(model, max_tokens=(ctx + 63) // 64 * 64 * slots, max_step_tokens=args.batch, profile=profile, cache_format=args.cache)
 
 
 def _describe(model, engine):
@@ -199,6 +199,7 @@ def build_parser():
         p.add_argument("--preset", help="a built-in shape with random weights instead of -m")
         p.add_argument("--random-seed", type=int, default=0)
         p.add_argument("--dtype", default="bf16", help="bf16 | f32 (f32: everything in true 32-bit)")
+        p.add_argument("--cache", choices=["int8", "fp8"], default=None, help="keep keys and values as 8-bit codes with a scale per row (default: in --dtype)")
         p.add_argument("--ctx", type=int, default=1024, help="max context per sequence")
         p.add_argument("--batch", type=int, default=8192, help="tokens per forward (longer steps are cut)")
         p.add_argument("--slots", type=int, default=8, help="sequences alive at once")

@@ -1613,19 +1613,21 @@ def _raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, kcache, vcache, k_scale, v_scale, nh, nkv, hd, err):
-    """`rope_kv_append` into the 8-bit cache: rotate q and k of the fused projection output in float32 (q back in place), write k and v
-    as codes and scales into their pages."""
+def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, kcache, vcache, k_scale, v_scale, nh, nkv, hd, err, q_out=None):
+    """`rope_kv_append` into the 8-bit cache: rotate q and k of the fused projection output in float32 (q back in place, or to `q_out`
+    [tokens, nh * hd] where given: `qkv` is then left as it was), write k and v as codes and scales into their pages."""
     what = "rope_quantize_append"
     _heads(nh, nkv, hd, what)
     code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
     if not qkv.is_contiguous() or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd or qkv.get_device() != device:
         raise KernelError(f"{what}: the projections must be contiguous rows of {(nh + 2 * nkv) * hd} numbers on the cache's device")
     T = qkv.shape[0]
+    if q_out is not None and (q_out.shape != (T, nh * hd) or q_out.dtype != qkv.dtype or not q_out.is_contiguous() or q_out.get_device() != device):
+        raise KernelError(f"{what}: q_out must be contiguous rows of {nh * hd} numbers, one per token, of the projections' type")
     _quant_tables(cos, sin, hd, device, what)
     _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
-    _check(_entry("edgelm_rope_quantize_append", "piipppp" "iippi" "pppp" "iiiipp")(
-        qkv.data_ptr(), _dt(qkv), code, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+    _check(_entry("edgelm_rope_quantize_append", "ppiipppp" "iippi" "pppp" "iiiipp")(
+        qkv.data_ptr(), q_out.data_ptr() if q_out is not None else None, _dt(qkv), code, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.stride(0),
         kcache.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
         T, nh, nkv, hd, err.data_ptr(), _raw_stream(device)), launches=1 if T else 0)
 

@@ -1,144 +1,234 @@
 // Writing the 8-bit cache and reading it back (the format: quant_cache.cuh).
 //
-//   rope_quantize_append   a step's queries rotated in place; its keys rotated and its values as they are, each row as codes and a
-//                          scale into its page.  A row is held by hd / 8 neighbouring lanes (rounded up to a power of two), each
-//                          with four numbers of the row's first half and their partners of the second: the rotation needs no
-//                          exchange, the row's largest magnitude log2(lanes) shuffles, and all reads and writes are pieces of 4
-//                          numbers.  Bound by memory: a number is read once and a code written once.
-//   quantized_rows         rows of given tokens as numbers.
+//   rope_quantize_append   a step's queries rotated (in place, or to rows of their own); its keys rotated and its values as they are,
+//                          each row as codes and a scale into its page.  A row is held by hd / 16 neighbouring lanes (rounded up to a
+//                          power of two), each with eight numbers of the row's first half and their partners of the second: the
+//                          rotation needs no exchange, the row's largest magnitude log2(lanes) shuffles, and all reads and writes
+//                          are pieces of 8 numbers.
+//   quantized_rows         rows of given tokens as numbers, 16 codes a lane.
+//
+// Bound by memory where there are many tokens, and there by the chain position -> sequence -> slot -> page -> row that a lane walks
+// before it may write (or read) a row: a warp stays with one token, walks the chain once, and has up to four rows' pieces a lane on
+// their way at a time.  With few tokens a lane has one piece, so that the token is spread over more warps.
+#include <type_traits>
+
 #include "quant_cache.cuh"
 
 namespace edgelm {
 
 constexpr int QA_THREADS = 256;
+constexpr int QA_MANY_PIECES = 4;
+constexpr int QA_MANY_TOKENS = 64;    // from here on QA_MANY_PIECES pieces a lane
 
-template <typename T, int FMT, int LANES>   // LANES: lanes of a row (a power of two, at least hd / 8)
+// Eight neighbouring numbers as they are stored.
+template <typename T> struct Piece8;
+template <> struct Piece8<__nv_bfloat16> {
+  uint4 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Piece8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The page of a token's position, or -1 (reported by one lane).
+__device__ __forceinline__ int page_of_token(int pos, int max_pos, int seq, const int32_t* seq_slot, const int32_t* page_table, int table_stride,
+                                             int n_pages, bool report, int* err) {
+  if (pos < 0 || pos >= max_pos) {
+    if (report) atomicOr(err, ERR_POSITION_RANGE);
+    return -1;
+  }
+  const int page = pos / PAGE < table_stride ? page_table[(size_t)seq_slot[seq] * table_stride + pos / PAGE] : -1;
+  if (page < 0 || page >= n_pages) {
+    if (report) atomicOr(err, ERR_PAGE_RANGE);
+    return -1;
+  }
+  return page;
+}
+
+template <typename T, int FMT, int LANES, int PIECES>   // LANES: lanes of a row (a power of two, at least hd / 16); PIECES a lane
 __global__ void __launch_bounds__(QA_THREADS)
-rope_quantize_append_kernel(T* __restrict__ qkv, const int32_t* __restrict__ tok_pos, const int32_t* __restrict__ tok_seq,
+rope_quantize_append_kernel(T* __restrict__ qkv, T* __restrict__ q_out, const int32_t* __restrict__ tok_pos, const int32_t* __restrict__ tok_seq,
                             const int32_t* __restrict__ seq_slot, const int32_t* __restrict__ page_table, int table_stride, int n_pages,
                             const float* __restrict__ cos_t, const float* __restrict__ sin_t, int max_pos, uint8_t* __restrict__ kcache,
                             uint8_t* __restrict__ vcache, float* __restrict__ k_scale, float* __restrict__ v_scale, int n_tokens, int nh,
-                            int nkv, int hd, int* __restrict__ err) {
+                            int nkv, int hd, int warps_per_token, int* __restrict__ err) {
+  constexpr int ROWS = 32 / LANES;      // of a warp at a time
   pdl_launch_dependents();
   pdl_wait();   // (launched as a programmatic dependent: the projections are the kernel before this one's)
-  const int rows = nh + 2 * nkv, half = hd >> 1;
-  const long long row = ((long long)blockIdx.x * QA_THREADS + threadIdx.x) / LANES;
-  const int part = threadIdx.x % LANES, j = part * 4;
-  const int t = (int)(row / rows), r = (int)(row - (long long)t * rows);
-  bool work = t < n_tokens;
-  const int pos = work ? tok_pos[t] : 0;
-  int page = 0;
-  if (work && (pos < 0 || pos >= max_pos)) {
-    if (part == 0 && r == 0) atomicOr(err, ERR_POSITION_RANGE);
-    work = false;
-  }
-  if (work) {
-    page = pos / PAGE < table_stride ? page_table[(size_t)seq_slot[tok_seq[t]] * table_stride + pos / PAGE] : -1;
-    if (page < 0 || page >= n_pages) {
-      if (part == 0 && r == 0) atomicOr(err, ERR_PAGE_RANGE);
-      work = false;
-    }
-  }
-  const bool mine = work && j < half;
-  T* src = qkv + (size_t)(work ? t : 0) * rows * hd + (size_t)r * hd + j;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-  if (mine) {
-    a = load_piece(src);
-    b = load_piece(src + half);
-    if (r < nh + nkv) {
-      const float4 c = *reinterpret_cast<const float4*>(cos_t + (size_t)pos * half + j), s = *reinterpret_cast<const float4*>(sin_t + (size_t)pos * half + j);
-      rotate_pair(a.x, b.x, c.x, s.x);
-      rotate_pair(a.y, b.y, c.y, s.y);
-      rotate_pair(a.z, b.z, c.z, s.z);
-      rotate_pair(a.w, b.w, c.w, s.w);
-    }
-  }
-  uint32_t most = max(max(max(magnitude_bits(a.x), magnitude_bits(a.y)), max(magnitude_bits(a.z), magnitude_bits(a.w))),
-                      max(max(magnitude_bits(b.x), magnitude_bits(b.y)), max(magnitude_bits(b.z), magnitude_bits(b.w))));
+  const int rows = nh + 2 * nkv, half = hd >> 1, lane = threadIdx.x & 31, part = lane % LANES, j = part * 8;
+  const int warp = blockIdx.x * (QA_THREADS / 32) + (threadIdx.x >> 5);
+  const int t = warp / warps_per_token, chunk = warp - t * warps_per_token;
+  if (t >= n_tokens) return;            // (whole warps)
+  const int row0 = chunk * ROWS * PIECES + lane / LANES;
+  T* src = qkv + (size_t)t * rows * hd + j;
+  Piece8<T> lo[PIECES], hi[PIECES];
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if (!mine) return;
-  if (r < nh) {
-    store_piece(src, a);
-    store_piece(src + half, b);
-    return;
+  for (int i = 0; i < PIECES; ++i) {
+    const int r = row0 + i * ROWS;
+    if (r < rows && j < half) {
+      lo[i].load(src + (size_t)r * hd);
+      hi[i].load(src + (size_t)r * hd + half);
+    }
   }
-  const RowScale rs = row_scale<FMT>(most);
-  const int h = r < nh + nkv ? r - nh : r - nh - nkv;
-  const size_t at = ((size_t)page * nkv + h) * PAGE + pos % PAGE;
-  uint8_t* codes = (r < nh + nkv ? kcache : vcache) + at * hd + j;
-  *reinterpret_cast<uint32_t*>(codes) = to_codes4<FMT>(a.x, a.y, a.z, a.w, rs.to_codes);
-  *reinterpret_cast<uint32_t*>(codes + half) = to_codes4<FMT>(b.x, b.y, b.z, b.w, rs.to_codes);
-  if (part == 0) (r < nh + nkv ? k_scale : v_scale)[at] = rs.scale;
+  const int pos = tok_pos[t];
+  const int page = page_of_token(pos, max_pos, tok_seq[t], seq_slot, page_table, table_stride, n_pages, lane == 0 && chunk == 0, err);
+  if (page < 0) return;                 // (whole warps: the token is the warp's)
+  float cs[8], sn[8];
+  if (j < half) {
+    Piece8<float> c;
+    c.load(cos_t + (size_t)pos * half + j);
+    c.get(cs);
+    c.load(sin_t + (size_t)pos * half + j);
+    c.get(sn);
+  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int r = row0 + i * ROWS;
+    const bool mine = r < rows && j < half;
+    float a[8] = {}, b[8] = {};
+    uint32_t most = 0;
+    if (mine) {
+      lo[i].get(a);
+      hi[i].get(b);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (r < nh + nkv) rotate_pair(a[k], b[k], cs[k], sn[k]);
+        most = max(most, max(magnitude_bits(a[k]), magnitude_bits(b[k])));
+      }
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (!mine) continue;
+    if (r < nh) {
+      T* dst = q_out ? q_out + ((size_t)t * nh + r) * hd + j : src + (size_t)r * hd;
+      store8(dst, a);
+      store8(dst + half, b);
+      continue;
+    }
+    const RowScale rs = row_scale<FMT>(most);
+    const bool is_v = r >= nh + nkv;
+    const size_t at = ((size_t)page * nkv + (is_v ? r - nh - nkv : r - nh)) * PAGE + pos % PAGE;
+    uint8_t* codes = (is_v ? vcache : kcache) + at * hd + j;
+    *reinterpret_cast<uint2*>(codes) = make_uint2(to_codes4<FMT>(a[0], a[1], a[2], a[3], rs.to_codes), to_codes4<FMT>(a[4], a[5], a[6], a[7], rs.to_codes));
+    *reinterpret_cast<uint2*>(codes + half) = make_uint2(to_codes4<FMT>(b[0], b[1], b[2], b[3], rs.to_codes), to_codes4<FMT>(b[4], b[5], b[6], b[7], rs.to_codes));
+    if (part == 0) (is_v ? v_scale : k_scale)[at] = rs.scale;
+  }
 }
 
-// keys[t], values[t] [nkv, hd] = the numbers that the cache holds for token t; a lane eight of them.
-template <typename T, int FMT>
+// keys[t], values[t] [nkv, hd] = the numbers that the cache holds for token t; a lane 16 of a row's at a time.
+template <typename T, int FMT, int PIECES>
 __global__ void __launch_bounds__(QA_THREADS)
 quantized_rows_kernel(const uint8_t* __restrict__ kcache, const uint8_t* __restrict__ vcache, const float* __restrict__ k_scale,
                       const float* __restrict__ v_scale, const int32_t* __restrict__ tok_pos, const int32_t* __restrict__ tok_seq,
                       const int32_t* __restrict__ seq_slot, const int32_t* __restrict__ page_table, int table_stride, int n_pages,
-                      T* __restrict__ keys, T* __restrict__ values, int n_tokens, int nkv, int hd, int* __restrict__ err) {
+                      T* __restrict__ keys, T* __restrict__ values, int n_tokens, int nkv, int hd, int warps_per_token, int* __restrict__ err) {
   pdl_launch_dependents();
   pdl_wait();
-  const int per_row = hd >> 3, per_token = 2 * nkv * per_row;
-  const long long i = (long long)blockIdx.x * QA_THREADS + threadIdx.x;
-  const int t = (int)(i / per_token);
+  const int per_row = hd >> 4, per_token = 2 * nkv * per_row, lane = threadIdx.x & 31;
+  const int warp = blockIdx.x * (QA_THREADS / 32) + (threadIdx.x >> 5);
+  const int t = warp / warps_per_token, chunk = warp - t * warps_per_token;
   if (t >= n_tokens) return;
-  const int it = (int)(i - (long long)t * per_token), row = it / per_row, d = (it - row * per_row) * 8;
-  const bool is_v = row >= nkv;
-  const int h = is_v ? row - nkv : row;
   const int pos = tok_pos[t];
-  int page = -1;
-  if (pos < 0) {
-    if (it == 0) atomicOr(err, ERR_POSITION_RANGE);
-  } else {
-    if (pos / PAGE < table_stride) page = page_table[(size_t)seq_slot[tok_seq[t]] * table_stride + pos / PAGE];
-    if (page < 0 || page >= n_pages) {
-      page = -1;
-      if (it == 0) atomicOr(err, ERR_PAGE_RANGE);
+  const int page = page_of_token(pos, 0x7fffffff, tok_seq[t], seq_slot, page_table, table_stride, n_pages, lane == 0 && chunk == 0, err);
+  const size_t first = ((size_t)max(page, 0) * nkv) * PAGE + max(pos, 0) % PAGE;
+  uint4 c[PIECES];
+  float scale[PIECES];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int it = (chunk * PIECES + i) * 32 + lane, row = it / per_row, d = (it - row * per_row) * 16;
+    c[i] = make_uint4(0, 0, 0, 0);
+    scale[i] = 0.f;                     // (a token that the cache cannot hold: zeros, and the error word says so)
+    if (it < per_token && page >= 0) {
+      const bool is_v = row >= nkv;
+      const size_t at = first + (size_t)(is_v ? row - nkv : row) * PAGE;
+      c[i] = *reinterpret_cast<const uint4*>((is_v ? vcache : kcache) + at * hd + d);
+      scale[i] = (is_v ? v_scale : k_scale)[at];
     }
   }
-  T* dst = (is_v ? values : keys) + ((size_t)t * nkv + h) * hd + d;
-  float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;     // (a token that the cache cannot hold: zeros, and the error word says so)
-  if (page >= 0) {
-    const size_t at = ((size_t)page * nkv + h) * PAGE + pos % PAGE;
-    const uint2 c = *reinterpret_cast<const uint2*>((is_v ? vcache : kcache) + at * hd + d);
-    const float s = (is_v ? v_scale : k_scale)[at];
-    uint32_t p0, p1, p2, p3;
-    codes_to_half<FMT>(c.x, p0, p1);
-    codes_to_half<FMT>(c.y, p2, p3);
-    const float2 f0 = half2_to_floats(p0), f1 = half2_to_floats(p1), f2 = half2_to_floats(p2), f3 = half2_to_floats(p3);
-    lo = make_float4(f0.x * s, f0.y * s, f1.x * s, f1.y * s);
-    hi = make_float4(f2.x * s, f2.y * s, f3.x * s, f3.y * s);
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int it = (chunk * PIECES + i) * 32 + lane, row = it / per_row, d = (it - row * per_row) * 16;
+    if (it >= per_token) break;
+    const bool is_v = row >= nkv;
+    T* dst = (is_v ? values : keys) + ((size_t)t * nkv + (is_v ? row - nkv : row)) * hd + d;
+    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x[8] = {};
+      if (page >= 0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t p0, p1;
+          codes_to_half<FMT>(w[2 * h + k], p0, p1);
+          const float2 f0 = half2_to_floats(p0), f1 = half2_to_floats(p1);
+          x[4 * k] = f0.x * scale[i];
+          x[4 * k + 1] = f0.y * scale[i];
+          x[4 * k + 2] = f1.x * scale[i];
+          x[4 * k + 3] = f1.y * scale[i];
+        }
+      }
+      store8(dst + 8 * h, x);
+    }
   }
-  store_piece(dst, lo);
-  store_piece(dst + 4, hi);
 }
 
 template <typename T, int FMT>
-static void launch_append(const void* qkv, const int32_t* tok_pos, const int32_t* tok_seq, const int32_t* seq_slot, const int32_t* page_table,
+static void launch_append(const void* qkv, void* q_out, const int32_t* tok_pos, const int32_t* tok_seq, const int32_t* seq_slot, const int32_t* page_table,
                           int table_stride, int n_pages, const float* cos_t, const float* sin_t, int max_pos, void* kc, void* vc, float* ks,
                           float* vs, int n_tokens, int nh, int nkv, int hd, int* err, cudaStream_t stream) {
-  const int lanes = hd / 8 <= 2 ? 2 : hd / 8 <= 4 ? 4 : hd / 8 <= 8 ? 8 : hd / 8 <= 16 ? 16 : 32;
-  const long long threads = (long long)n_tokens * (nh + 2 * nkv) * lanes;
-  auto go = [&](auto kern) {
-    launch_pdl(pdl_bit_for_tokens(n_tokens), kern, dim3((unsigned)((threads + QA_THREADS - 1) / QA_THREADS)), dim3(QA_THREADS), (size_t)0, stream,
-               (T*)const_cast<void*>(qkv), tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, cos_t, sin_t, max_pos, (uint8_t*)kc,
-               (uint8_t*)vc, ks, vs, n_tokens, nh, nkv, hd, err);
+  const bool many = n_tokens >= QA_MANY_TOKENS;
+  auto go = [&](auto kern, int lanes) {
+    const int per_warp = 32 / lanes * (many ? QA_MANY_PIECES : 1), warps = (nh + 2 * nkv + per_warp - 1) / per_warp;
+    launch_pdl(pdl_bit_for_tokens(n_tokens), kern, dim3((unsigned)(((long long)n_tokens * warps + QA_THREADS / 32 - 1) / (QA_THREADS / 32))), dim3(QA_THREADS),
+               (size_t)0, stream, (T*)const_cast<void*>(qkv), (T*)q_out, tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, cos_t, sin_t, max_pos,
+               (uint8_t*)kc, (uint8_t*)vc, ks, vs, n_tokens, nh, nkv, hd, warps, err);
   };
-  if (lanes == 2) go(rope_quantize_append_kernel<T, FMT, 2>);
-  else if (lanes == 4) go(rope_quantize_append_kernel<T, FMT, 4>);
-  else if (lanes == 8) go(rope_quantize_append_kernel<T, FMT, 8>);
-  else if (lanes == 16) go(rope_quantize_append_kernel<T, FMT, 16>);
-  else go(rope_quantize_append_kernel<T, FMT, 32>);
+  auto lanes = [&](auto n) {
+    constexpr int L = decltype(n)::value;
+    many ? go(rope_quantize_append_kernel<T, FMT, L, QA_MANY_PIECES>, L) : go(rope_quantize_append_kernel<T, FMT, L, 1>, L);
+  };
+  if (hd <= 16) lanes(std::integral_constant<int, 1>{});
+  else if (hd <= 32) lanes(std::integral_constant<int, 2>{});
+  else if (hd <= 64) lanes(std::integral_constant<int, 4>{});
+  else if (hd <= 128) lanes(std::integral_constant<int, 8>{});
+  else lanes(std::integral_constant<int, 16>{});
 }
 
 }  // namespace edgelm
 
 using namespace edgelm;
 
-extern "C" int edgelm_rope_quantize_append(void* qkv, int dtype, int format, const int32_t* tok_pos, const int32_t* tok_seq, const int32_t* seq_slot,
+// q_out: rows [n_tokens, nh hd] for the rotated queries, or null: back in place.
+extern "C" int edgelm_rope_quantize_append(void* qkv, void* q_out, int dtype, int format, const int32_t* tok_pos, const int32_t* tok_seq, const int32_t* seq_slot,
                                            const int32_t* page_table, int table_stride, int n_pages, const float* cos_t, const float* sin_t,
                                            int max_pos, void* kcache, void* vcache, float* k_scale, float* v_scale, int n_tokens, int nh, int nkv,
                                            int hd, int* err, cudaStream_t stream) {
@@ -146,10 +236,10 @@ extern "C" int edgelm_rope_quantize_append(void* qkv, int dtype, int format, con
   EL_REFUSE(n_tokens > 0 && nh > 0 && nkv > 0, "rope_quantize_append: bad sizes");
   EL_REFUSE(hd >= 16 && hd <= 256 && hd % 16 == 0, "rope_quantize_append: head size %d (takes 16..256 in steps of 16)", hd);
   EL_REFUSE((format == QF_INT8 || format == QF_FP8) && (dtype == DT_F32 || dtype == DT_BF16), "rope_quantize_append: format %d, dtype %d", format, dtype);
-  EL_REFUSE((uintptr_t)qkv % 16 == 0 && (uintptr_t)cos_t % 16 == 0 && (uintptr_t)sin_t % 16 == 0 && (uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0,
+  EL_REFUSE((uintptr_t)qkv % 16 == 0 && (uintptr_t)q_out % 16 == 0 && (uintptr_t)cos_t % 16 == 0 && (uintptr_t)sin_t % 16 == 0 && (uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0,
             "rope_quantize_append: rows must start on 16-byte boundaries");
-  EL_REFUSE((long long)n_tokens * (nh + 2 * nkv) * 32 / QA_THREADS < 0x7fffffffLL, "rope_quantize_append: grid too large");
-  auto go = [&](auto fn) { fn(qkv, tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, cos_t, sin_t, max_pos, kcache, vcache, k_scale, v_scale,
+  EL_REFUSE((long long)n_tokens * (nh + 2 * nkv) < 0x7fffffffLL, "rope_quantize_append: grid too large");
+  auto go = [&](auto fn) { fn(qkv, q_out, tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, cos_t, sin_t, max_pos, kcache, vcache, k_scale, v_scale,
                               n_tokens, nh, nkv, hd, err, stream); };
   if (dtype == DT_F32) format == QF_INT8 ? go(launch_append<float, QF_INT8>) : go(launch_append<float, QF_FP8>);
   else format == QF_INT8 ? go(launch_append<__nv_bfloat16, QF_INT8>) : go(launch_append<__nv_bfloat16, QF_FP8>);
@@ -167,16 +257,22 @@ extern "C" int edgelm_quantized_rows(const void* kcache, const void* vcache, con
   EL_REFUSE((format == QF_INT8 || format == QF_FP8) && (dtype == DT_F32 || dtype == DT_BF16), "quantized_rows: format %d, dtype %d", format, dtype);
   EL_REFUSE((uintptr_t)keys % 16 == 0 && (uintptr_t)values % 16 == 0 && (uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0,
             "quantized_rows: rows must start on 16-byte boundaries");
-  const long long threads = (long long)n_tokens * 2 * nkv * (hd / 8);
-  const dim3 grid((unsigned)((threads + QA_THREADS - 1) / QA_THREADS));
+  EL_REFUSE((long long)n_tokens * 2 * nkv < 0x7fffffffLL, "quantized_rows: grid too large");
+  const bool many = n_tokens >= QA_MANY_TOKENS;
+  const int per_warp = 32 * (many ? QA_MANY_PIECES : 1), warps = (2 * nkv * (hd / 16) + per_warp - 1) / per_warp;
+  const dim3 grid((unsigned)(((long long)n_tokens * warps + QA_THREADS / 32 - 1) / (QA_THREADS / 32)));
   auto go = [&](auto kern, auto* out) {
     using T = std::remove_pointer_t<decltype(out)>;
     launch_pdl(pdl_bit_for_tokens(n_tokens), kern, grid, dim3(QA_THREADS), (size_t)0, stream, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale,
-               tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, (T*)keys, (T*)values, n_tokens, nkv, hd, err);
+               tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, (T*)keys, (T*)values, n_tokens, nkv, hd, warps, err);
   };
-  if (dtype == DT_F32) format == QF_INT8 ? go(quantized_rows_kernel<float, QF_INT8>, (float*)nullptr) : go(quantized_rows_kernel<float, QF_FP8>, (float*)nullptr);
-  else format == QF_INT8 ? go(quantized_rows_kernel<__nv_bfloat16, QF_INT8>, (__nv_bfloat16*)nullptr)
-                         : go(quantized_rows_kernel<__nv_bfloat16, QF_FP8>, (__nv_bfloat16*)nullptr);
+  auto type = [&](auto* out) {
+    using T = std::remove_pointer_t<decltype(out)>;
+    if (format == QF_INT8) many ? go(quantized_rows_kernel<T, QF_INT8, QA_MANY_PIECES>, out) : go(quantized_rows_kernel<T, QF_INT8, 1>, out);
+    else many ? go(quantized_rows_kernel<T, QF_FP8, QA_MANY_PIECES>, out) : go(quantized_rows_kernel<T, QF_FP8, 1>, out);
+  };
+  if (dtype == DT_F32) type((float*)nullptr);
+  else type((__nv_bfloat16*)nullptr);
   EL_LAUNCH_CHECK("quantized_rows");
   return 0;
 }

@@ -73,14 +73,17 @@ def load_model(model_dir, dtype="bfloat16", device="cuda:0"):
 
 class Engine:
     def __init__(self, model: DecoderModel, max_tokens, max_step_tokens=8192, max_seqs=None, profile=False,
-                 use_graphs=True):
+                 use_graphs=True, cache_format=None):
+        """`cache_format`: None (keys and values in the compute dtype), or "int8" or "fp8": 8-bit codes with a float32 scale per row of
+        head_dim numbers, for models whose attention reads them (half of a bfloat16 cache's bytes, a quarter of a float32 one's)."""
         ops.require_device()
         if model.device is None:
             raise EngineError("the model has no weights yet (load them first)")
         self.model, self.device = model, model.device
         self.plan = model.plan
+        model.check_cache_format(cache_format)
         self.cache = SequenceCache(model.cache_needs(), max_tokens, self.plan.max_positions, dtype=model.dtype,
-                                   device=self.device, max_seqs=max_seqs)
+                                   device=self.device, max_seqs=max_seqs, format=cache_format)
         self.max_step_tokens = int(min(max_step_tokens, max(64, self.cache.n_pages * 64)))
         self.max_step_seqs = min(self.cache.n_slots, self.max_step_tokens)
         props = torch.cuda.get_device_properties(self.device)
@@ -98,7 +101,7 @@ class Engine:
         self._err_copied = torch.cuda.Event()
         self._err_pending = False
         self.buffers = BatchBuffers(self.max_step_tokens, self.max_step_seqs, self.cache.kv_groups, self.max_step_tokens,
-                                    self.device, tile_sizes=model.tile_sizes())
+                                    self.device, tile_sizes=model.tile_sizes(cache_format))
         self.profiler = Profiler() if profile else None
         self.ctx = StepContext(self.ws, self.err, self.device, self.n_sms, self.profiler)
         self.sampler = DeviceSampler(self.cache.n_slots, self.device)

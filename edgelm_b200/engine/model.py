@@ -9,7 +9,7 @@ import torch
 
 from ..config.base import ConfigError, ModelPlan
 from ..parts import registry as part_registry
-from ..parts.base import nbytes
+from ..parts.base import KVNeed, NeedSet, StateNeed, nbytes
 
 
 class DecoderModel:
@@ -87,9 +87,23 @@ class DecoderModel:
         """Whether every part allows its steps to be replayed from a CUDA graph."""
         return all(p.graph_safe for p in [self.embedding, self.final_norm, self.head] + self.layers)
 
-    def tile_sizes(self):
-        """Every attention tile size a layer will ask the step for."""
-        return sorted({t for l in self.layers for t in l.tile_sizes()})
+    def tile_sizes(self, cache_format=None):
+        """Every attention tile size a layer will ask the step for (with a cache kept in an 8-bit format: then)."""
+        if cache_format is None:
+            return sorted({t for l in self.layers for t in l.tile_sizes()})
+        from ..csrc import ops
+        return sorted({t for l in self.layers for t in l.quantized_tile_sizes()} | {ops.QUANT_PREFILL_TILE})
+
+    def check_cache_format(self, cache_format):
+        """Refuse an 8-bit format that a layer reading another run's cache does not know (the layers that keep a cache of
+        their own say so in their needs)."""
+        def known(need):
+            return need is not None and all(known(n) for _, n in need.items) if isinstance(need, NeedSet) else \
+                isinstance(need, StateNeed) or (isinstance(need, KVNeed) and cache_format in need.formats)
+        if cache_format is not None:
+            for i, e in enumerate(self.schedule):
+                if e.reads_cache_of is not None and not known(self.layers[e.layer].cache_need()):
+                    raise ConfigError(f"schedule entry {i} reads another entry's cache, but not one kept as {cache_format} codes")
 
     def workspace_bytes(self, n_tokens, n_seqs, n_want):
         d = self.plan.hidden_size

@@ -4,6 +4,9 @@ q, k, v = h Wq^T, h Wk^T, h Wv^T (no bias; one matrix product over the three wei
 rotary positions on q and k; k and v appended to the cache; for query head h and key head
 h // (heads / kv_heads): softmax((q . K_j) / sqrt(head_dim)) over j <= the token's position,
 times V; then x += a Wo^T (adarsh-sgh/edgelm src/kernels_ref.cpp:100-141, tools/elm.py:126-139).
+
+The cache may be kept in an 8-bit format (`KVNeed.formats`): keys and values are then rounded to codes as they are written, and
+attention reads the codes, a token's own among them, so that prompts cut into several steps see the same numbers.
 """
 import math
 
@@ -82,7 +85,12 @@ class Attention(Part):
         return (self.w_qkv,)
 
     def cache_need(self):
-        return KVNeed(self.nkv, self.hd, self.window)
+        # (an 8-bit cache is written with the position encoding, so the encoding has to know how)
+        formats = tuple(ops.QUANT_FORMATS) if hasattr(self.positions, "encode_and_quantize") and hasattr(self.positions, "rotation_tables") else ()
+        return KVNeed(self.nkv, self.hd, self.window, formats=formats)
+
+    def quantized_tile_sizes(self):
+        return (ops.QUANT_PREFILL_TILE,)
 
     # Steps whose longest sequence brings fewer new tokens than this stay on the mma.sync kernel (tiles of 64 rows):
     # measured at 9 heads of 64 (32 heads): 128 new tokens 4.6 (5.0) us against 5.7 (5.8) us on tcgen05, 256 tokens
@@ -140,12 +148,36 @@ class Attention(Part):
                 ops.attn_decode(qkv, a, cache.k, cache.v, table, ctx.seq_index, ctx.seq_pos, ctx.n_seqs, self.nh, self.nkv,
                                 self.hd, self.scale, splits, part_o, part_ml, err=ctx.err, window=self.window, meta_ready=ready)
 
+    def _mix_quantized(self, ctx, h, qkv, a, cache, table):
+        """`a` <- the attention of the step's tokens over a cache in an 8-bit format."""
+        kept = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+        with ctx.prof("qkv_proj"):
+            linear.matmul(ctx, h, self.w_qkv, qkv, prefetch=(self.w_o,))
+        if ctx.all_single:
+            # one token per sequence: rotation, append and attention in one kernel
+            with ctx.prof("attn_decode"):
+                ops.attn_decode_rope_quantized(qkv, a, *kept, table, ctx.seq_index, ctx.seq_pos, *self.positions.rotation_tables(), ctx.n_seqs, self.nh,
+                                               self.nkv, self.hd, self.scale, err=ctx.err, window=self.window,
+                                               meta_ready=getattr(ctx, "metadata_precedes_kernels", False))
+            return
+        with ctx.prof("rope_quantize_append"):
+            self.positions.encode_and_quantize(ctx, qkv, cache, self.nh, self.nkv)
+        tiles = ctx.tiles(ops.QUANT_PREFILL_TILE)
+        with ctx.prof("attn_prefill"):
+            ops.attn_prefill_quantized(qkv, a, *kept, table, ctx.seq_index, tiles.seq, tiles.tok0, tiles.ntok, tiles.pos0, tiles.count, self.nh, self.nkv,
+                                       self.hd, self.scale, err=ctx.err, window=self.window, max_keys=max(p + n for p, n in zip(ctx.seq_first_positions, ctx.seq_lengths)))
+
     def forward(self, ctx, h, x, cache):
         T = h.shape[0]
         ws = ctx.ws
         qkv = ws.alloc((T, (self.nh + 2 * self.nkv) * self.hd), self.dtype)
         a = ws.alloc((T, self.nh * self.hd), self.dtype)
         table = ctx.page_table(cache.group)
+        if cache.group.format is not None:
+            self._mix_quantized(ctx, h, qkv, a, cache, table)
+            with ctx.prof("o_proj_residual"):
+                linear.matmul(ctx, a, self.w_o, x, epilogue=linear.EPI_RESIDUAL, residual=x, prefetch=ctx.weights_after)
+            return
         tables = self.positions.rotation_tables() if hasattr(self.positions, "rotation_tables") else None
         encoded = False
         if not ctx.all_single and hasattr(self.positions, "project_encode_append"):

@@ -32,7 +32,7 @@ input in the compute dtype.  Mixers and feed-forwards ADD into x, so that the re
 be fused into their last matrix product.  `ctx` is the step's StepContext: positions, sequence
 boundaries, page tables, workspace; tokens of all sequences are packed along the first axis.
 """
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Tuple
 
 import torch
@@ -45,13 +45,16 @@ class KVNeed:
     row per block of `pool` consecutive positions (the block's mean, written by the mixer when the block is full),
     kept in the page that holds the block's last position: `CacheEntry.pooled_k / pooled_v`.  `values_in_keys`: no
     value rows of their own are kept (a latent that is key and value at once: the mixer reads its values out of the
-    key rows); `CacheEntry.v` is then None."""
+    key rows); `CacheEntry.v` is then None.  `formats`: the 8-bit formats ("int8", "fp8") that the mixer's kernels read and write
+    in place of the compute dtype, if the engine's cache is to be kept in one (`CacheEntry.k_scale / v_scale`); it says nothing
+    about what is kept, so needs that differ in it alone share a group."""
     n_kv_heads: int
     head_dim: int
     window: int = None
     v_head_dim: int = None
     pool: int = None
     values_in_keys: bool = False
+    formats: Tuple[str, ...] = field(default=(), compare=False)
 
 
 @dataclass(frozen=True)
@@ -109,6 +112,10 @@ class Part:
         """Sizes of attention tiles (`ctx.tiles(n)`) this part will ask for: the engine lays them out
         with the step's metadata, which is what lets a whole step be replayed from a CUDA graph."""
         return ()
+
+    def quantized_tile_sizes(self):
+        """`tile_sizes` where the cache is kept in an 8-bit format."""
+        return tuple(self.tile_sizes())
 
 
 def as_matrix(t, dtype, device):

@@ -54,6 +54,9 @@ class PreNormBlock(Part):
     def tile_sizes(self):
         return tuple(self.mixer.tile_sizes())
 
+    def quantized_tile_sizes(self):
+        return tuple(self.mixer.quantized_tile_sizes())
+
     @property
     def graph_safe(self):
         return all(p.graph_safe for p in self.parts)
@@ -205,6 +208,9 @@ class SublayerNormBlock(Part):
     def tile_sizes(self):
         return tuple(self.mixer.tile_sizes())
 
+    def quantized_tile_sizes(self):
+        return tuple(self.mixer.quantized_tile_sizes())
+
     @property
     def graph_safe(self):
         return all(p.graph_safe for p in self.parts)
@@ -323,6 +329,9 @@ class HyperBlock(Part):
 
     def tile_sizes(self):
         return tuple(self.mixer.tile_sizes())
+
+    def quantized_tile_sizes(self):
+        return tuple(self.mixer.quantized_tile_sizes())
 
     @property
     def graph_safe(self):

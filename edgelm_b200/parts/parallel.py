@@ -65,6 +65,9 @@ class ParallelMixers(Part):
     def tile_sizes(self):
         return tuple(self.left.tile_sizes()) + tuple(self.right.tile_sizes())
 
+    def quantized_tile_sizes(self):
+        return tuple(self.left.quantized_tile_sizes()) + tuple(self.right.quantized_tile_sizes())
+
     def cache_need(self):
         return NeedSet.of(left=self.left.cache_need(), right=self.right.cache_need())
 

@@ -61,6 +61,11 @@ class RotaryPositions(Part):
         ops.rope_kv_append(qkv, ctx.tok_pos, ctx.tok_seq, ctx.seq_index, ctx.page_table(cache.group), self.cos, self.sin,
                            cache.k, cache.v, n_heads, n_kv_heads, self.head_dim, ctx.err)
 
+    def encode_and_quantize(self, ctx, qkv, cache, n_heads, n_kv_heads):
+        """`encode_and_append` into a cache kept in an 8-bit format."""
+        ops.rope_quantize_append(qkv, ctx.tok_pos, ctx.tok_seq, ctx.seq_index, ctx.page_table(cache.group), self.cos, self.sin,
+                                 cache.k, cache.v, cache.k_scale, cache.v_scale, n_heads, n_kv_heads, self.head_dim, ctx.err)
+
 
 def rotary_frequencies(dims, base, scaling=None):
     """Float64 frequencies f_i = base^(-2i / dims), i < dims / 2, for kernels that form position * f_i themselves.

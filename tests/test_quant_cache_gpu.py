@@ -94,10 +94,14 @@ def test_append_writes_what_the_format_says(fmt, dtype, hd, nh, nkv):
         want[scales][page, :, pos.long() % 64] = s
     want_q, rest = turned[:, :nh].to(qkv.dtype), x[:, nh:].clone()
     err = word()
+    # the queries to rows of their own first: the projections stay as they were
+    other, before, q_out = {k: v.clone() for k, v in cache.items()}, qkv.clone(), torch.zeros((len(pos), nh * hd), dtype=qkv.dtype, device=DEV)
+    ops.rope_quantize_append(qkv, pos, seq, slot, table, cos, sin, *cache_args(other), nh, nkv, hd, err, q_out=q_out)
+    assert same(qkv, before) and same(q_out, want_q.reshape(len(pos), -1).contiguous())
     ops.rope_quantize_append(qkv, pos, seq, slot, table, cos, sin, *cache_args(cache), nh, nkv, hd, err)
     assert int(err) == 0
     for k in want:
-        assert same(cache[k], want[k]), k
+        assert same(cache[k], want[k]) and same(other[k], want[k]), k
     assert same(qkv.view(-1, nh + 2 * nkv, hd)[:, :nh].contiguous(), want_q.contiguous())
     assert same(qkv.view(-1, nh + 2 * nkv, hd)[:, nh:].float(), rest)
     # and back
@@ -108,6 +112,29 @@ def test_append_writes_what_the_format_says(fmt, dtype, hd, nh, nkv):
         for got, codes, scales in ((keys, "k", "ks"), (values, "v", "vs")):
             n = cache[codes].view(torch.int8)[page, :, at].view(cache[codes].dtype).float() * cache[scales][page, :, at][..., None]
             assert same(got.float(), n.to(out).float())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_append_of_few_tokens_writes_what_that_of_many_writes(fmt, dtype):
+    nh, nkv, hd = 15, 5, 64
+    qkv, pos, seq = step([80], [80], nh, nkv, hd, DTYPES[dtype], 5)
+    cos, sin = ref.tables(80, hd, DEV)
+    caches, queries, rows = [], [], []
+    for piece in (80, 7):
+        cache, table = ref.make_cache(fmt, nkv, hd, [80], DEV, 3)
+        x = qkv.clone()
+        keys, values = (torch.empty((80, nkv, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        for a in range(0, 80, piece):
+            part = slice(a, min(80, a + piece))
+            ops.rope_quantize_append(x[part], pos[part], seq[part], i32([0]), table, cos, sin, *cache_args(cache), nh, nkv, hd, word())
+        for a in range(0, 80, piece):
+            part = slice(a, min(80, a + piece))
+            ops.quantized_rows(*cache_args(cache), pos[part], seq[part], i32([0]), table, keys[part], values[part], word())
+        caches.append(cache)
+        queries.append(x)
+        rows.append((keys, values))
+    assert all(same(caches[0][k], caches[1][k]) for k in caches[0]) and same(*queries) and same(rows[0][0], rows[1][0]) and same(rows[0][1], rows[1][1])
 
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
