@@ -144,7 +144,7 @@ def prepare(case, seed):
          "table": table.to(DEVICE), "pos": dev(pos), "seq": dev(seq), "slot": dev(range(B)), "seq_pos": dev([t - 1 for t in totals]),
          "tiles": [dev([t[i] for t in tiles]) for i in range(4)], "cos": cos, "sin": sin, "B": B, "T": T, "most": max(totals),
          "scale": 1.0 / math.sqrt(hd), "err": torch.zeros(1, dtype=torch.int32, device=DEVICE),
-         "out": torch.empty((T, nh * hd), dtype=dtype, device=DEVICE), "step_qkv": torch.empty((T, (nh + 2 * nkv) * hd), dtype=dtype, device=DEVICE),
+         "out": torch.empty((T, nh * hd), dtype=dtype, device=DEVICE),
          "row_keys": torch.empty((T, nkv, hd), dtype=torch.bfloat16, device=DEVICE),
          "row_values": torch.empty((T, nkv, hd), dtype=torch.bfloat16, device=DEVICE)}
     # where a padded query row [sequence, place] of a prompt step lies among the packed ones
@@ -237,10 +237,9 @@ def run(s):
                                        s["scale"], err=s["err"], window=c["window"], max_keys=s["most"])
             return s["out"]
         if c["op"] == "write":
-            s["step_qkv"].copy_(s["qkv"])      # (the append rotates the queries in place, and the pass can be made again)
-            ops.rope_quantize_append(s["step_qkv"], s["pos"], s["seq"], s["slot"], s["table"], s["cos"], s["sin"], *cache, nh, nkv, hd, s["err"])
+            ops.rope_quantize_append(s["qkv"], s["pos"], s["seq"], s["slot"], s["table"], s["cos"], s["sin"], *cache, nh, nkv, hd, s["err"], q_out=s["out"])
             ops.quantized_rows(*cache, s["pos"], s["seq"], s["slot"], s["table"], s["row_keys"], s["row_values"], s["err"])
-            return s["step_qkv"][:, :nh * hd], s["row_keys"], s["row_values"]
+            return s["out"], s["row_keys"], s["row_values"]
         ops.attn_decode_rope_quantized(s["qkv"], s["out"], *cache, s["table"], s["slot"], s["seq_pos"], s["cos"], s["sin"], s["B"], nh, nkv, hd,
                                        s["scale"], err=s["err"], window=c["window"])
         ops.quantized_rows(*cache, s["seq_pos"], s["slot"], s["slot"], s["table"], s["row_keys"], s["row_values"], s["err"])
