@@ -144,7 +144,7 @@ def prepare(case, seed):
          "table": table.to(DEVICE), "pos": dev(pos), "seq": dev(seq), "slot": dev(range(B)), "seq_pos": dev([t - 1 for t in totals]),
          "tiles": [dev([t[i] for t in tiles]) for i in range(4)], "cos": cos, "sin": sin, "B": B, "T": T, "most": max(totals),
          "scale": 1.0 / math.sqrt(hd), "err": torch.zeros(1, dtype=torch.int32, device=DEVICE),
-         "out": torch.empty((T, nh * hd), dtype=dtype, device=DEVICE),
+         "out": torch.empty((T, nh * hd), dtype=dtype, device=DEVICE), "step_qkv": torch.empty((T, (nh + 2 * nkv) * hd), dtype=dtype, device=DEVICE),
          "row_keys": torch.empty((T, nkv, hd), dtype=torch.bfloat16, device=DEVICE),
          "row_values": torch.empty((T, nkv, hd), dtype=torch.bfloat16, device=DEVICE)}
     # where a padded query row [sequence, place] of a prompt step lies among the packed ones
