@@ -7,6 +7,11 @@ int launch_decode_quant_int8(const QuantDecodeArgs& p, int dtype, int hd, int n_
 int launch_decode_quant_fp8(const QuantDecodeArgs& p, int dtype, int hd, int n_seqs, int n_splits, int warps, cudaStream_t stream);
 int launch_prefill_quant_int8(const QuantPrefillArgs& p, int dtype, int hd, int n_tiles, int n_splits, cudaStream_t stream);
 int launch_prefill_quant_fp8(const QuantPrefillArgs& p, int dtype, int hd, int n_tiles, int n_splits, cudaStream_t stream);
+bool prefill_quant_tc_takes(const void* q, long long ldq, const void* out, long long ldo, int dtype, int hd);
+int launch_prefill_quant_tc(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache, const float* k_scale,
+                            const float* v_scale, int format, const int32_t* page_table, int table_stride, int n_pages, const int32_t* seq_slot,
+                            const int32_t* tile_seq, const int32_t* tile_tok0, const int32_t* tile_ntok, const int32_t* tile_pos0, int n_tiles,
+                            int max_tile_tokens, int nh, int nkv, int hd, float scale, int window, int* err, cudaStream_t stream);
 }  // namespace edgelm
 
 using namespace edgelm;
@@ -46,12 +51,12 @@ extern "C" int edgelm_attn_decode_quantized(const void* q, long long ldq, void* 
 }
 
 // New tokens, any number a sequence, as tiles of at most `max_tile_tokens` (up to 128) consecutive tokens of one sequence; their keys and
-// values are in the cache already.  n_splits: blocks that share a row tile's keys, 1 to 8.
+// values are in the cache already.  n_splits: blocks that share a row tile's keys, 1 to 8 (mma.sync).  form: 0 by sizes, 1 mma.sync, 2 tcgen05.
 extern "C" int edgelm_attn_prefill_quantized(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache,
                                              const float* k_scale, const float* v_scale, int dtype, int format, const int32_t* page_table,
                                              int table_stride, int n_pages, const int32_t* seq_slot, const int32_t* tile_seq, const int32_t* tile_tok0,
                                              const int32_t* tile_ntok, const int32_t* tile_pos0, int n_tiles, int max_tile_tokens, int nh, int nkv,
-                                             int hd, float scale, int n_splits, int window, int* err, cudaStream_t stream) {
+                                             int hd, float scale, int n_splits, int window, int form, int* err, cudaStream_t stream) {
   if (n_tiles == 0) return 0;
   const char* who = "attn_prefill_quantized";
   EL_REFUSE(nh > 0 && nkv > 0 && nh % nkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, nh, nkv);
@@ -64,6 +69,16 @@ extern "C" int edgelm_attn_prefill_quantized(const void* q, long long ldq, void*
             "%s: the cache must start on 16-byte boundaries", who);
   EL_REFUSE((uintptr_t)q % 16 == 0 && ldq % 4 == 0, "%s: query rows must start on a 16-byte boundary, a multiple of 4 numbers apart", who);
   EL_REFUSE((uintptr_t)out % 8 == 0 && ldo % 2 == 0, "%s: output rows must start on 8-byte boundaries", who);
+  EL_REFUSE(form >= 0 && form <= 2, "%s: form %d", who, form);
+  const bool tc = form != 1 && err != nullptr && prefill_quant_tc_takes(q, ldq, out, ldo, dtype, hd);
+  EL_REFUSE(form != 2 || tc, "%s: these operands are not taken on tcgen05 (bfloat16, head size 64 or 128, 16-byte rows, an error word)", who);
+  if (form == 2 || (tc && max_tile_tokens * (nh / nkv) >= 128)) {
+    const int rc = launch_prefill_quant_tc(q, ldq, out, ldo, kcache, vcache, k_scale, v_scale, format, page_table, table_stride, n_pages, seq_slot, tile_seq,
+                                           tile_tok0, tile_ntok, tile_pos0, n_tiles, max_tile_tokens, nh, nkv, hd, scale, window, err, stream);
+    if (rc) return rc;
+    EL_LAUNCH_CHECK(who);
+    return 0;
+  }
   const int per_tile = (max_tile_tokens * (nh / nkv) + QP_ROWS - 1) / QP_ROWS;
   EL_REFUSE(nkv <= 65535 && (long long)n_tiles * per_tile <= 65535, "%s: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", who, n_tiles, per_tile);
   const QuantPrefillArgs p = {q, out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok,

@@ -1,0 +1,479 @@
+// Causal attention of many new tokens over the 8-bit cache on the fifth-generation tensor cores (tcgen05): bfloat16 models, head
+// sizes 64 and 128.  The other head sizes, float32 models and short steps stay on mma.sync (attention_quant_prefill.cuh).
+//
+// The tensor cores take float16 operands, so the codes become float16 on the chip, keys and values (every code is exact), and the scales
+// are applied to scores and weights as attention_quant.cuh says, a key at a time.  M moves only when a row's largest x has outgrown it
+// by 2^8, so the operand's factor is 2^-40 here: a weight is under 2^15 as an operand.  (Values times their scale beside the largest of 32
+// neighbours, as float16, would spare a shared-memory read in two; but then a row would lose digits to neighbours that it must not see.)
+// A value row that is no number makes its key's factor one that is none: who sees the key sees NaN, and nothing but numbers enters a
+// product.
+//
+// A block takes 128 (token, query head) rows of one kv head, token-major, and walks the keys that they see in blocks of two pages.
+// Roles: warp 0 brings codes and scales (bulk copies, two stages); warps 4 to 7 turn them into swizzled float16 tiles (keys K-major, values
+// MN-major as they lie) and key factors; warp 1 issues S = Q K^T, warp 2 O += P V with P out of tensor memory; warps 8 to 15 are the
+// softmax, two threads a row, 64 keys of the block each, which share a row's reference through shared memory.  S has two buffers of 128
+// columns, so that S of block j + 1 is computed beside the softmax of block j; the weights go back over the scores that they came from.
+// Every wait is bounded; where one runs out the block reports it, writes not-a-numbers and waits for what it has in flight before
+// it gives its memory back.
+#include <math_constants.h>
+
+#include "attention_quant.cuh"
+#include "tc_common.cuh"
+
+namespace edgelm {
+
+constexpr int QT_ROWS = 128, QT_KEYS = 128, QT_THREADS = 512, QT_SOFT_WARPS = 8, QT_CONVERTERS = 4;
+constexpr int QT_TILE = 128 * 128;             // bytes of 128 rows of 64 float16
+constexpr float QT_LAZY = 8.f;
+constexpr float QT_OPERAND = 0.00390625f, QT_OPERAND_BACK = 1099511627776.f;    // 2^-8 (to AQ_OPERAND's 2^-32), 2^40
+
+template <int HD> struct QtSizes {
+  static constexpr int KC = HD / 64;                          // tiles of 64 dims
+  static constexpr int KS = 2, VS = KC == 1 ? 2 : 1;          // stages of keys and values (shared memory has room for one of values at 128)
+  static constexpr int CODES = QT_KEYS * (2 * HD + 8);        // a stage: key codes, value codes, key scales, value scales
+  static constexpr int KEY_DATA = 4 * QT_KEYS * 4;            // a block's u log2(e) scale, e, f, 2^-e of every key; four blocks' worth
+  static constexpr int smem = 1024 + (KC + KS * KC + VS * KC) * QT_TILE + 2 * CODES + 4 * KEY_DATA + (4 + 2) * QT_ROWS * 4 + 256;
+};
+
+// Instruction descriptor of kind::f16 with float16 operands: D float32, both K-major, M x N.
+__host__ __device__ constexpr uint32_t qt_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+struct QuantTcArgs {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const uint8_t *kcache, *vcache;
+  const float *k_scale, *v_scale;
+  const int32_t *page_table, *seq_slot, *tile_seq, *tile_tok0, *tile_ntok, *tile_pos0;
+  int* err;
+  long long ldq, ldo;
+  int table_stride, n_pages, nh, nkv, window, blocks_per_tile;
+  float scale;
+};
+
+__device__ __forceinline__ uint64_t qt_pair(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 qt_unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t qt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t qt_mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t qt_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ void qt_tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// A block's last wait for what it has in flight, bounded and without a report (the wait that ran out before has made one)
+__device__ __forceinline__ void qt_drain(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try(bar, parity) && clock64() - t0 < TC_WAIT_CYCLES) {}
+}
+// where eight dims d .. d + 7 of row r lie in tiles of 128 rows of 64 float16 numbers, swizzled
+__device__ __forceinline__ uint8_t* qt_place(uint8_t* tiles, int r, int d) { return tiles + d / 64 * QT_TILE + r * 128 + (((d % 64 / 8) ^ (r & 7)) << 4); }
+
+template <int HD, int FMT>
+__global__ void __launch_bounds__(QT_THREADS, 1)
+attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
+  using Z = QtSizes<HD>;
+  constexpr int KC = Z::KC, KS = Z::KS, VS = Z::VS;
+  extern __shared__ uint8_t qt_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(qt_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* q_s = smem;                             // [KC][128 rows][128 bytes]
+  uint8_t* k_s = q_s + KC * QT_TILE;               // [KS][KC][128 keys][128 bytes]
+  uint8_t* v_s = k_s + KS * KC * QT_TILE;          // [VS][KC][128 keys][128 bytes]
+  uint8_t* codes = v_s + VS * KC * QT_TILE;        // [2][CODES]
+  uint8_t* key_data = codes + 2 * Z::CODES;        // [4][KEY_DATA]
+  float* row_max = reinterpret_cast<float*>(key_data + 4 * Z::KEY_DATA);      // [block & 1][half of its keys][128 rows]
+  float* row_sum = row_max + 4 * QT_ROWS;          // [half of the keys][128 rows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(row_sum + 2 * QT_ROWS);
+  uint64_t *q_ready = bars, *c_full = bars + 1, *c_empty = c_full + 2, *k_full = c_empty + 2, *k_empty = k_full + KS, *v_full = k_empty + KS;
+  uint64_t *v_empty = v_full + VS, *s_ready = v_empty + VS, *p_ready = s_ready + 2, *o_done = p_ready + 2;
+  uint64_t* d_full = o_done + 2;                   // [4] key factors
+  uint64_t* all_done = d_full + 4;                 // both issuers' MMAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (uint64_t* b = bars; b < all_done; ++b)
+      mbar_init(smem_u32(b), b == q_ready || (b >= p_ready && b < o_done) ? QT_SOFT_WARPS
+                             : (b >= c_empty && b < k_empty) || (b >= v_full && b < v_empty) || b >= d_full ? QT_CONVERTERS : 1);
+    mbar_init(smem_u32(all_done), 2);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();      // (behind the allocation: a block of the next kernel must not hold tensor memory that this one waits for)
+  pdl_wait();
+
+  const int g = a.nh / a.nkv, kvh = blockIdx.x, at = gridDim.y - 1 - blockIdx.y;      // (tiles of the most keys first)
+  const int tile = at / a.blocks_per_tile, row_base = (at - tile * a.blocks_per_tile) * QT_ROWS;
+  const int tok0 = a.tile_tok0[tile], rows_total = a.tile_ntok[tile] * g, pos0 = a.tile_pos0[tile];
+  const int rows = min(QT_ROWS, rows_total - row_base);
+  const int first_pos = pos0 + row_base / g, last_pos = pos0 + (row_base + max(rows, 1) - 1) / g;
+  const int n_keys = last_pos + 1, page0 = a.window > 0 ? max(0, first_pos - a.window + 1) / PAGE : 0, n_pg = (n_keys + PAGE - 1) / PAGE - page0;
+  const int n_blk = rows > 0 ? (n_pg + 1) / 2 : 0;     // (no rows: a block of a tile that has fewer tokens than the longest)
+  auto key_of = [&](int j) { return (page0 + 2 * j) * PAGE; };
+  constexpr uint32_t S_COLS = 128, O_COL = 256;
+  auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait_parked(smem_u32(bar), (uint32_t)parity, abort_flag, a.err)); };
+
+  if (n_blk == 0) {
+  } else if (warp == 0) {
+    // ---- codes and scales: lanes 0 to 3 the block's first page, 4 to 7 its second
+    const int32_t* pages = a.page_table + (size_t)a.seq_slot[a.tile_seq[tile]] * a.table_stride;
+    auto page_of = [&](int j) {
+      const int i = page0 + 2 * j + (lane >> 2);
+      int page = lane < 8 && j < n_blk && 2 * j + (lane >> 2) < n_pg ? (i < a.table_stride ? pages[i] : -1) : 0;
+      if (page < 0 || page >= a.n_pages) {
+        atomicOr(a.err, ERR_PAGE_RANGE);
+        page = 0;                                  // (reported; some page is read in its place)
+      }
+      return page;
+    };
+    int issued = 0, page = page_of(0);
+    for (int j = 0; j < n_blk; ++j) {
+      const int st = j & 1, both = 2 * j + 1 < n_pg ? 2 : 1;
+      const int next = page_of(j + 1);
+      if (j >= 2 && !wait(&c_empty[st], (j >> 1 & 1) ^ 1)) break;
+      const uint32_t bar = smem_u32(&c_full[st]), dst = smem_u32(codes + st * Z::CODES);
+      if (lane == 0) mbar_expect_tx(bar, both * PAGE * (2 * HD + 8));
+      __syncwarp();
+      if (lane < 4 * both) {
+        const int h = lane >> 2, what = lane & 3;
+        const size_t row = ((size_t)page * a.nkv + kvh) * PAGE;
+        if (what < 2) aq_bulk(dst + what * QT_KEYS * HD + h * PAGE * HD, (what ? a.vcache : a.kcache) + row * HD, PAGE * HD, bar);
+        else aq_bulk(dst + 2 * QT_KEYS * HD + (what - 2) * QT_KEYS * 4 + h * PAGE * 4, (what == 2 ? a.k_scale : a.v_scale) + row, PAGE * 4, bar);
+      }
+      issued = j + 1;
+      page = next;
+      __syncwarp();
+    }
+    // (also where a wait ran out: no copy may be on its way when the block's memory is given back)
+    for (int i = max(0, issued - 2); i < issued; ++i) qt_drain(smem_u32(&c_full[i & 1]), i >> 1 & 1);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = qt_idesc(QT_ROWS, QT_KEYS);
+    const bool leader = elect_one();
+    const uint64_t dq = umma_desc(smem_u32(q_s));
+    bool ok = wait(q_ready, 0);
+    for (int j = 0; j < n_blk && ok; ++j) {
+      const int b = j & 1, st = j % KS;
+      if (j >= 2) ok = wait(&o_done[b], (j >> 1) - 1 & 1);            // (the block before last has left this buffer)
+      if (ok) ok = wait(&k_full[st], j / KS & 1);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t dk = umma_desc(smem_u32(k_s + st * KC * QT_TILE));
+      if (leader) {
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s)
+          umma_f16(tmem + b * S_COLS, dq + (s / 4 * QT_TILE >> 4) + 2 * (s % 4), dk + (s / 4 * QT_TILE >> 4) + 2 * (s % 4), idesc, s != 0);
+        umma_commit(smem_u32(&s_ready[b]));
+        umma_commit(smem_u32(&k_empty[st]));
+      }
+      __syncwarp();
+    }
+    if (leader) umma_commit(smem_u32(all_done));
+    __syncwarp();
+    qt_drain(smem_u32(all_done), 0);
+  } else if (warp == 2) {
+    constexpr uint32_t idesc = qt_idesc(QT_ROWS, 64) | (1u << 16);    // B (the values) is MN-major
+    const bool leader = elect_one();
+    bool ok = true;
+    for (int j = 0; j < n_blk && ok; ++j) {
+      const int b = j & 1, st = j % VS;
+      ok = wait(&v_full[st], j / VS & 1) && wait(&p_ready[b], j >> 1 & 1);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t dv = umma_desc(smem_u32(v_s + st * KC * QT_TILE));
+      if (leader) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int s = 0; s < 8; ++s)                                 // 16 keys: 8 columns of the weights of half s / 4
+            umma_f16_ts(tmem + O_COL + c * 64, tmem + b * S_COLS + s / 4 * 64 + s % 4 * 8, (uint32_t)dv + (c * QT_TILE + s * 16 * 128 >> 4), (uint32_t)(dv >> 32), idesc,
+                        j > 0 || s != 0);
+        umma_commit(smem_u32(&o_done[b]));
+        umma_commit(smem_u32(&v_empty[st]));
+      }
+      __syncwarp();
+    }
+    if (leader) umma_commit(smem_u32(all_done));
+    __syncwarp();
+    qt_drain(smem_u32(all_done), 0);
+  } else if (warp >= 4 && warp < 8) {
+    // ---- 32 keys a warp: their factors, and their codes as float16 tiles
+    constexpr int PER_ROW = HD / 16, ROWS = 32 / PER_ROW;             // pieces of 16 codes; rows of a pass
+    const int cw = warp - 4, sub = lane / PER_ROW, d = lane % PER_ROW * 16;
+    for (int j = 0; j < n_blk; ++j) {
+      const int cs = j & 1, ks = j % KS, vs = j % VS;
+      if (!wait(&c_full[cs], j >> 1 & 1)) break;
+      if (j >= KS && !wait(&k_empty[ks], (j / KS & 1) ^ 1)) break;    // (and with S of block j - 2 done, the softmax is done with block j - 4's factors)
+      const uint8_t* src = codes + cs * Z::CODES + cw * 32 * HD;
+      const float* scales = reinterpret_cast<const float*>(codes + cs * Z::CODES + 2 * QT_KEYS * HD) + cw * 32 + lane;
+      const bool there = key_of(j) + cw * 32 + lane < n_keys;
+      const float u = there ? scales[0] : 0.f, v = there ? scales[QT_KEYS] : 0.f;
+      const bool fine = (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u;
+      const ValueScale vsc = value_scale(fine ? v : 0.f);
+      float* kd = reinterpret_cast<float*>(key_data + (j & 3) * Z::KEY_DATA) + cw * 32 + lane;
+      kd[0] = fine ? u * (a.scale * AQ_LOG2E) : CUDART_NAN_F;
+      kd[QT_KEYS] = vsc.e;
+      kd[2 * QT_KEYS] = vsc.f * QT_OPERAND;
+      kd[3 * QT_KEYS] = vsc.undo;
+#pragma unroll
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const int r = i * ROWS + sub;
+        const uint4 c = *reinterpret_cast<const uint4*>(src + r * HD + d);
+        uint4 lo, hi;
+        codes_to_half<FMT>(c.x, lo.x, lo.y);
+        codes_to_half<FMT>(c.y, lo.z, lo.w);
+        codes_to_half<FMT>(c.z, hi.x, hi.y);
+        codes_to_half<FMT>(c.w, hi.z, hi.w);
+        uint8_t* dst = k_s + ks * KC * QT_TILE;
+        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d)) = lo;
+        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d + 8)) = hi;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&k_full[ks]));
+        mbar_arrive(smem_u32(&d_full[j & 3]));
+      }
+      if (j >= VS && !wait(&v_empty[vs], (j / VS & 1) ^ 1)) break;
+#pragma unroll
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const int r = i * ROWS + sub;
+        uint4 c = *reinterpret_cast<const uint4*>(src + QT_KEYS * HD + r * HD + d);
+        if (key_of(j) + cw * 32 + r >= n_keys) c = make_uint4(0, 0, 0, 0);      // whatever lies there, it meets weights of zero as zero
+        uint4 lo, hi;
+        codes_to_half<FMT>(c.x, lo.x, lo.y);
+        codes_to_half<FMT>(c.y, lo.z, lo.w);
+        codes_to_half<FMT>(c.z, hi.x, hi.y);
+        codes_to_half<FMT>(c.w, hi.z, hi.w);
+        uint8_t* dst = v_s + vs * KC * QT_TILE;
+        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d)) = lo;
+        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d + 8)) = hi;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&v_full[vs]));
+        mbar_arrive(smem_u32(&c_empty[cs]));
+      }
+    }
+  } else if (warp >= 8) {
+    const int half = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int rr = row_base + row, tok = rr / g;
+    const bool mine = row < rows;
+    // ---- this thread's half of its query row as float16 numbers, lifted by a power of two (exact)
+    float qf;
+    {
+      uint4 v[HD / 16];
+      uint32_t most = 0;
+      const __nv_bfloat16* src = a.q + (size_t)(tok0 + tok) * a.ldq + (size_t)(kvh * g + rr - tok * g) * HD + half * (HD / 2);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        v[i] = mine ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) most = max(most, max(w[k] << 16 & 0x7fffffffu, w[k] & 0x7fff0000u));
+      }
+      row_max[half * QT_ROWS + row] = __uint_as_float(most);
+      asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
+      most = max(most, __float_as_uint(row_max[(half ^ 1) * QT_ROWS + row]));
+      asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");      // (both have read, before the maxima are written over)
+      const float lift = query_lift(most);
+      qf = 1.0f / lift;
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = aq_pack(__uint_as_float(w[k] << 16) * lift, __uint_as_float(w[k] & 0xffff0000u) * lift);
+        *reinterpret_cast<uint4*>(qt_place(q_s, row, half * (HD / 2) + 8 * i)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(q_ready));
+    }
+    const uint64_t qf2 = qt_pair(qf, qf);
+    const int pos = mine ? pos0 + tok : last_pos;
+    float m = -CUDART_INF_F, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n_blk; ++j) {              // (also behind a wait that ran out: the row's other thread may be at the exchange)
+      const int b = j & 1, key0 = key_of(j) + half * 64;
+      const uint32_t s_addr = tmem + lanes + b * S_COLS + half * 64;
+      const ulonglong2* kd = reinterpret_cast<const ulonglong2*>(key_data + (j & 3) * Z::KEY_DATA) + half * 16;      // four keys' u; 32 further their e, f, 2^-e
+      if (ok) ok = wait(&d_full[j & 3], j >> 2 & 1) && wait(&s_ready[b], j >> 1 & 1);
+      uint64_t x[32];                              // pairs of neighbouring keys
+      float mx = -CUDART_INF_F;
+      if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        uint32_t r[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {              // a group of 32 keys
+          tmem_ld32(s_addr + c * 32, r);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const ulonglong2 uu = kd[c * 8 + i], ee = kd[32 + c * 8 + i];
+            x[c * 16 + 2 * i] = qt_fma2(qt_mul2(qt_pair(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), uu.x), qf2, ee.x);
+            x[c * 16 + 2 * i + 1] = qt_fma2(qt_mul2(qt_pair(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), uu.y), qf2, ee.y);
+          }
+        }
+        if (key0 + 63 > first_pos || (a.window > 0 && key0 <= last_pos - a.window)) {
+          const int hi = pos - key0, lo = a.window > 0 ? hi - a.window : -1;      // keys lo + 1 .. hi of the thread's 64
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float2 v = qt_unpair(x[i]);
+            x[i] = qt_pair(2 * i <= hi && 2 * i > lo ? v.x : -CUDART_INF_F, 2 * i + 1 <= hi && 2 * i + 1 > lo ? v.y : -CUDART_INF_F);
+          }
+        }
+        float mx1 = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 v = qt_unpair(x[i]), w = qt_unpair(x[i + 1]);
+          mx = fmaxf(mx, fmaxf(v.x, v.y));
+          mx1 = fmaxf(mx1, fmaxf(w.x, w.y));
+        }
+        mx = fmaxf(mx, mx1);
+      }
+      row_max[(b * 2 + half) * QT_ROWS + row] = mx;
+      asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");      // the row's two threads (warps w and w + 4)
+      if (!ok) continue;
+      mx = fmaxf(mx, row_max[(b * 2 + (half ^ 1)) * QT_ROWS + row]);
+      float rescale = 1.f;
+      if (j == 0) {
+        m = mx;
+      } else if (mx > m + QT_LAZY) {
+        rescale = aq_exp2(m - mx);                 // (0 if the row has seen no key so far)
+        m = mx;
+        l *= rescale;
+      }
+      if (__any_sync(0xffffffffu, rescale != 1.f)) {       // (rare after the first blocks; both warps of the rows take it)
+        ok = wait(&o_done[b ^ 1], (j - 1) >> 1 & 1);
+        if (!ok) continue;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < HD / 2; c += 8) {
+          uint32_t o[8];
+          const uint32_t o_addr = tmem + lanes + O_COL + half * (HD / 2) + c;
+          tmem_ld8(o_addr, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * rescale);
+          qt_tmem_st8(o_addr, o);
+        }
+      }
+      const float ref = m == -CUDART_INF_F ? 0.f : m;
+      const uint64_t bias = qt_pair(AQ_LIFT - ref, AQ_LIFT - ref);
+      uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        uint32_t w[8];
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {           // four keys
+          const ulonglong2 ff = kd[64 + (i + k) / 2], un = kd[96 + (i + k) / 2];
+          const float2 y0 = qt_unpair(qt_add2(x[i + k], bias)), y1 = qt_unpair(qt_add2(x[i + k + 1], bias));
+          const uint64_t t0 = qt_pair(aq_exp2(y0.x), aq_exp2(y0.y)), t1 = qt_pair(aq_exp2(y1.x), aq_exp2(y1.y));
+          sum0 = qt_fma2(t0, un.x, sum0);
+          sum1 = qt_fma2(t1, un.y, sum1);
+          const float2 p0 = qt_unpair(qt_mul2(t0, ff.x)), p1 = qt_unpair(qt_mul2(t1, ff.y));
+          w[k] = aq_pack(p0.x, p0.y);
+          w[k + 1] = aq_pack(p1.x, p1.y);
+        }
+        qt_tmem_st8(s_addr + i, w);
+      }
+      const float2 sum = qt_unpair(qt_add2(sum0, sum1));
+      l += sum.x + sum.y;
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&p_ready[b]));
+    }
+    if (ok) ok = wait(&o_done[(n_blk - 1) & 1], (n_blk - 1) >> 1 & 1);
+    row_sum[half * QT_ROWS + row] = l;
+    asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
+    float inv = QT_OPERAND_BACK / (row_sum[row] + row_sum[QT_ROWS + row]);
+    if (!ok) inv = CUDART_NAN_F;                   // a wait that ran out: nothing that could pass for a result
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    __nv_bfloat16* dst = a.out + (size_t)(tok0 + tok) * a.ldo + (size_t)(kvh * g + rr - tok * g) * HD + half * (HD / 2);
+#pragma unroll
+    for (int c = 0; c < HD / 2; c += 32) {
+      uint32_t o[32];
+      tmem_ld32(tmem + lanes + O_COL + half * (HD / 2) + c, o);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      if (!mine) continue;
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
+          h[k] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+    __syncwarp();
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+template <int HD, int FMT>
+static int launch_quant_tc(const QuantTcArgs& a, int n_tiles, cudaStream_t stream) {
+  constexpr int smem = QtSizes<HD>::smem;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  auto kern = attn_prefill_quant_tc_kernel<HD, FMT>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  EL_REFUSE(e == cudaSuccess, "attn_prefill_quantized: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
+  launch_pdl(16, kern, dim3(a.nkv, n_tiles * a.blocks_per_tile), dim3(QT_THREADS), (size_t)smem, stream, a);
+  return 0;
+}
+
+// Rows of the operands are checked by the entry point (attention_quant.cu); this form also wants 16-byte rows of queries and outputs.
+bool prefill_quant_tc_takes(const void* q, long long ldq, const void* out, long long ldo, int dtype, int hd) {
+  return dtype == DT_BF16 && (hd == 64 || hd == 128) && (uintptr_t)q % 16 == 0 && ldq % 8 == 0 && (uintptr_t)out % 16 == 0 && ldo % 8 == 0;
+}
+
+int launch_prefill_quant_tc(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache, const float* k_scale,
+                            const float* v_scale, int format, const int32_t* page_table, int table_stride, int n_pages, const int32_t* seq_slot,
+                            const int32_t* tile_seq, const int32_t* tile_tok0, const int32_t* tile_ntok, const int32_t* tile_pos0, int n_tiles,
+                            int max_tile_tokens, int nh, int nkv, int hd, float scale, int window, int* err, cudaStream_t stream) {
+  const int per_tile = (max_tile_tokens * (nh / nkv) + QT_ROWS - 1) / QT_ROWS;
+  EL_REFUSE((long long)n_tiles * per_tile <= 65535, "attn_prefill_quantized: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", n_tiles, per_tile);
+  const QuantTcArgs a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot,
+                         tile_seq, tile_tok0, tile_ntok, tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, scale};
+  if (hd == 64) return format == QF_INT8 ? launch_quant_tc<64, QF_INT8>(a, n_tiles, stream) : launch_quant_tc<64, QF_FP8>(a, n_tiles, stream);
+  return format == QF_INT8 ? launch_quant_tc<128, QF_INT8>(a, n_tiles, stream) : launch_quant_tc<128, QF_FP8>(a, n_tiles, stream);
+}
+
+}  // namespace edgelm

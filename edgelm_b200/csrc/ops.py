@@ -1713,10 +1713,11 @@ def quantized_prefill_splits(n_blocks, hd, max_keys, n_sms=148):
 
 
 def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok, tile_pos0, n_tiles, nh, nkv,
-                           hd, scale, err=None, window=0, max_keys=0, n_splits=None):
+                           hd, scale, err=None, window=0, max_keys=0, n_splits=None, form=0):
     """`attn_prefill` over the 8-bit cache: causal attention of new tokens (any number per sequence), as tiles of at most
     QUANT_PREFILL_TILE consecutive tokens of one sequence; the tokens' own keys and values are in the cache.  `max_keys`: the longest
-    sequence's keys, if the caller knows them (0: the page table's width), by which the blocks that share keys are counted."""
+    sequence's keys, if the caller knows them (0: the page table's width), by which the blocks that share keys are counted.
+    `form`: 0 by sizes, 1 on mma.sync, 2 on tcgen05 (bfloat16, head size 64 or 128, with the error word)."""
     what = "attn_prefill_quantized"
     _heads(nh, nkv, hd, what)
     code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
@@ -1730,8 +1731,8 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     if n_splits is None:
         keys = max_keys or page_table.shape[1] * PAGE
         n_splits = quantized_prefill_splits(nkv * n_tiles * -(-most * (nh // nkv) // 64), hd, min(keys, window + most) if window > 0 else keys)
-    _check(_entry("edgelm_attn_prefill_quantized", "plplpppp" "iipii" "ppppp" "iiiii" "fiipp")(
+    _check(_entry("edgelm_attn_prefill_quantized", "plplpppp" "iipii" "ppppp" "iiiii" "fiiipp")(
         qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _dt(qkv),
         code, page_table.data_ptr(), page_table.stride(0), kcache.shape[0], seq_slot.data_ptr(), tile_seq.data_ptr(), tile_tok0.data_ptr(),
-        tile_ntok.data_ptr(), tile_pos0.data_ptr(), n_tiles, most, nh, nkv, hd, scale, n_splits, window, err.data_ptr() if err is not None else None,
+        tile_ntok.data_ptr(), tile_pos0.data_ptr(), n_tiles, most, nh, nkv, hd, scale, n_splits, window, form, err.data_ptr() if err is not None else None,
         _raw_stream(device)), launches=1 if n_tiles else 0)

@@ -19,7 +19,7 @@ def tiles_of(totals, news, size=128):
     return [i32(r[i] for r in rows) for i in range(4)], len(rows)
 
 
-def prompt_case(fmt, dtype, nh, nkv, hd, totals, news, window=0, splits=None, seed=1, spoil=True, change=None, size=128, max_keys=0, pad=0):
+def prompt_case(fmt, dtype, nh, nkv, hd, totals, news, window=0, splits=None, seed=1, spoil=True, change=None, size=128, max_keys=0, pad=0, form=0):
     dtype = DTYPES[dtype]
     cache, table = ref.make_cache(fmt, nkv, hd, totals, DEV, seed, k_size=1.5)
     if spoil:     # what lies behind a sequence's end is not its own: no number at all
@@ -40,7 +40,7 @@ def prompt_case(fmt, dtype, nh, nkv, hd, totals, news, window=0, splits=None, se
     err, scale = word(), 1 / math.sqrt(hd)
     tiles, n_tiles = tiles_of(totals, news, size)
     ops.attn_prefill_quantized(q, out[:, :nh * hd], *cache_args(cache), table, i32(range(len(totals))), *tiles, n_tiles, nh, nkv, hd, scale, err=err, window=window,
-                               max_keys=max_keys, n_splits=splits)
+                               max_keys=max_keys, n_splits=splits, form=form)
     assert int(err) == 0 and bool((out[:, nh * hd:] == 3.0).all())
     for k in before:
         assert same(before[k], cache[k])
@@ -62,7 +62,20 @@ TOTALS, NEWS = [1, 17, 64, 65, 200, 400, 300], [1, 17, 64, 2, 200, 129, 1]
 @pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 4, 64), (4, 1, 128), (3, 3, 32), (6, 2, 96), (2, 1, 16), (5, 1, 48), (3, 1, 80), (2, 2, 256), (12, 1, 64),
                                        (24, 2, 112), (7, 1, 192), (2, 1, 208), (2, 2, 144)])
 def test_prompt_heads_and_lengths(fmt, dtype, nh, nkv, hd):
+    prompt_case(fmt, dtype, nh, nkv, hd, TOTALS, NEWS, form=1)
     prompt_case(fmt, dtype, nh, nkv, hd, TOTALS, NEWS)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 4, 64), (12, 1, 64), (4, 1, 128), (3, 3, 128), (32, 2, 128)])
+def test_prompt_on_tcgen05(fmt, nh, nkv, hd):
+    prompt_case(fmt, "bf16", nh, nkv, hd, [1], [1], form=2)
+    prompt_case(fmt, "bf16", nh, nkv, hd, [17, 64], [17, 64], form=2)
+    prompt_case(fmt, "bf16", nh, nkv, hd, TOTALS, NEWS, form=2)
+    prompt_case(fmt, "bf16", nh, nkv, hd, [128, 1300, 129], [128, 700, 65], form=2)
+    prompt_case(fmt, "bf16", nh, nkv, hd, TOTALS, NEWS, form=2, size=50, pad=40)
+    for window in (1, 64, 65, 130, 300, 5000):
+        prompt_case(fmt, "bf16", nh, nkv, hd, TOTALS + [900], NEWS + [500], window=window, form=2)
 
 
 @pytest.mark.parametrize("splits", [1, 2, 3, 8])
@@ -98,7 +111,8 @@ def test_prompt_scales_of_all_sizes(fmt, dtype):
         cache["vs"].mul_((10.0 ** (torch.rand(cache["vs"].shape, generator=torch.Generator().manual_seed(9)) * 40 - 20)).to(DEV))
         cache["v"].view(torch.int8)[:, :, ::7] = 0
         cache["vs"][:, :, ::7] = 2.0 ** -60 / ref.TOP[fmt]
-    prompt_case(fmt, dtype, 9, 3, 64, [200, 70], [200, 7], change=change, spoil=False)
+    for form in (1, 2) if dtype == "bf16" else (1,):
+        prompt_case(fmt, dtype, 9, 3, 64, [200, 70], [200, 7], change=change, spoil=False, form=form)
 
 
 @pytest.mark.parametrize("splits", [1, 4])
@@ -108,8 +122,8 @@ def test_prompt_a_row_that_is_no_number_reaches_who_sees_it(splits):
         cache["v"].view(torch.int8)[int(table[0, 1]), 0, 5] = 0
         cache["ks"][int(table[0, 0]), 1, 3] = float("nan")       # key of position 3, kv head 1
         cache["k"].view(torch.int8)[int(table[0, 0]), 1, 3] = 0
-    for window in (0, 50):
-        out = prompt_case("fp8", "bf16", 4, 2, 64, [200], [200], change=change, spoil=False, splits=splits, window=window)
+    for window, form, hd in ((0, 1, 64), (50, 1, 64), (0, 2, 64), (50, 2, 64), (0, 2, 128)):
+        out = prompt_case("fp8", "bf16", 4, 2, hd, [200], [200], change=change, spoil=False, splits=splits, window=window, form=form)
         nan = torch.isnan(out).all(-1).cpu()
         p = torch.arange(200)
         first = (p >= 69) & ((p < 69 + window) if window else p >= 0)
@@ -143,4 +157,8 @@ def test_prompt_pages_that_are_not_there_are_reported():
         err = word()
         q = torch.randn((20, 128), device=DEV)
         ops.attn_prefill_quantized(q, torch.empty_like(q), *cache_args(cache), table, i32([0]), *tiles, n, 2, 1, 64, 0.125, err=err)
+        assert int(err) == 4
+        err.zero_()
+        q = q.bfloat16()
+        ops.attn_prefill_quantized(q, torch.empty_like(q), *cache_args(cache), table, i32([0]), *tiles, n, 2, 1, 64, 0.125, err=err, form=2)
         assert int(err) == 4

@@ -75,11 +75,11 @@ def test_the_library_refuses_too():
     for bad, word in (({"nh": 3}, "multiple"), ({"hd": 20}, "head size"), ({"fmt": 2}, "format"), ({"dtype": 5}, "dtype"), ({"splits": 17}, "splits"),
                       ({"splits": 0}, "splits"), ({"window": -1}, "window"), ({"cos": 256}, "tables"), ({"n_seqs": 70000}, "sequences"), ({"k": 264}, "16-byte")):
         assert go(**bad) < 0 and word in message(), (bad, message())
-    prefill = ops._entry("edgelm_attn_prefill_quantized", "plplpppp" "iipii" "ppppp" "iiiii" "fiipp")
+    prefill = ops._entry("edgelm_attn_prefill_quantized", "plplpppp" "iipii" "ppppp" "iiiii" "fiiipp")
 
-    def go2(dtype=0, fmt=0, n_tiles=1, most=128, nh=4, nkv=2, hd=64, splits=1, window=0, q=256, ldq=512):
-        return prefill(q, ldq, 256, 512, 256, 256, 256, 256, dtype, fmt, 256, 1, 1, 256, 256, 256, 256, 256, n_tiles, most, nh, nkv, hd, 0.1, splits, window, None, None)
+    def go2(dtype=0, fmt=0, n_tiles=1, most=128, nh=4, nkv=2, hd=64, splits=1, window=0, q=256, ldq=512, form=0):
+        return prefill(q, ldq, 256, 512, 256, 256, 256, 256, dtype, fmt, 256, 1, 1, 256, 256, 256, 256, 256, n_tiles, most, nh, nkv, hd, 0.1, splits, window, form, None, None)
     assert go2(n_tiles=0) == 0
     for bad, word in (({"nh": 3}, "multiple"), ({"hd": 20}, "head size"), ({"fmt": 2}, "format"), ({"most": 129}, "tokens"), ({"splits": 9}, "splits"),
-                      ({"window": -1}, "window"), ({"q": 264}, "16-byte"), ({"ldq": 510}, "multiple of 4"), ({"n_tiles": 60000, "nh": 8}, "65,535")):
+                      ({"window": -1}, "window"), ({"form": 3}, "form"), ({"form": 2}, "tcgen05"), ({"q": 264}, "16-byte"), ({"ldq": 510}, "multiple of 4"), ({"n_tiles": 60000, "nh": 8}, "65,535")):
         assert go2(**bad) < 0 and word in message(), (bad, message())
