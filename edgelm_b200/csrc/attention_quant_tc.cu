@@ -1,18 +1,22 @@
 // Causal attention of many new tokens over the 8-bit cache on the fifth-generation tensor cores (tcgen05): bfloat16 models, head
 // sizes 64 and 128.  The other head sizes, float32 models and short steps stay on mma.sync (attention_quant_prefill.cuh).
 //
-// The tensor cores take float16 operands, so the codes become float16 on the chip, keys and values (every code is exact), and the scales
-// are applied to scores and weights as attention_quant.cuh says, a key at a time.  M moves only when a row's largest x has outgrown it
-// by 2^8, so the operand's factor is 2^-40 here: a weight is under 2^15 as an operand.  (Values times their scale beside the largest of 32
-// neighbours, as float16, would spare a shared-memory read in two; but then a row would lose digits to neighbours that it must not see.)
-// A value row that is no number makes its key's factor one that is none: who sees the key sees NaN, and nothing but numbers enters a
-// product.
+// The tensor cores take float16 operands, so the codes become float16 on the chip.  Scales are applied 32 keys (a group) at a time: with
+// 2^k and 2^e the largest powers of two in the group's key and value scales, the tiles hold a_j (u_j / 2^k) and c_j (v_j / 2^e), one more
+// rounding to 11 bits each, and   x_ij = log2(e) scale 2^k (q_i . tile_j) + e,   t_ij = 2^(x_ij - M_i + 46),
+// out_i = 2^40 sum (t_ij 2^-40) (tile_j) / sum t_ij 2^-e   (attention_quant.cuh, with one e a group).  A softmax thread has one group: two
+// numbers for 32 scores.  (Scales applied a key at a time cost a thread four shared-memory reads for four scores, 16 bytes to every lane
+// though all lanes read the same: 2,048 clocks a block, twice its exponentials; 2,048 tokens of 32 heads of 64: 82 us.)
+// Where a group's key or value scales differ by more than 2^8 the tiles hold its codes as they are and the thread takes the slow way,
+// scales a key at a time: a row must not lose digits to a neighbour that it may not even see.  A row that is no number makes its key's
+// tile one of not-a-numbers (or, the slow way, its factor): who sees the key sees NaN, and only numbers enter the product with the values.
+// M moves only when a row's largest x has outgrown it by 2^8, so a weight is at most 2^15 as an operand.
 //
 // A block takes 128 (token, query head) rows of one kv head, token-major, and walks the keys that they see in blocks of two pages.
 // Roles: warp 0 brings codes and scales (bulk copies, two stages); warps 4 to 7 turn them into swizzled float16 tiles (keys K-major, values
-// MN-major as they lie) and key factors; warp 1 issues S = Q K^T, warp 2 O += P V with P out of tensor memory; warps 8 to 15 are the
-// softmax, two threads a row, 64 keys of the block each, which share a row's reference through shared memory.  S has two buffers of 128
-// columns, so that S of block j + 1 is computed beside the softmax of block j; the weights go back over the scores that they came from.
+// MN-major as they lie) and factors; warp 1 issues S = Q K^T, warp 2 O += P V with P out of tensor memory; warps 8 to 23 are the
+// softmax, four threads a row, a group each, which share the row's reference through shared memory.  S has two buffers of 128 columns,
+// so that S of block j + 1 is computed beside the softmax of block j; the weights go back over the scores that they came from.
 // Every wait is bounded; where one runs out the block reports it, writes not-a-numbers and waits for what it has in flight before
 // it gives its memory back.
 #include <math_constants.h>
@@ -22,17 +26,19 @@
 
 namespace edgelm {
 
-constexpr int QT_ROWS = 128, QT_KEYS = 128, QT_THREADS = 512, QT_SOFT_WARPS = 8, QT_CONVERTERS = 4;
+constexpr int QT_ROWS = 128, QT_KEYS = 128, QT_THREADS = 768, QT_SOFT_WARPS = 16, QT_GROUPS = 4, QT_CONVERTERS = 4;
 constexpr int QT_TILE = 128 * 128;             // bytes of 128 rows of 64 float16
 constexpr float QT_LAZY = 8.f;
-constexpr float QT_OPERAND = 0.00390625f, QT_OPERAND_BACK = 1099511627776.f;    // 2^-8 (to AQ_OPERAND's 2^-32), 2^40
+constexpr int QT_SPREAD = 8;                   // powers of two between the scales of a group that tiles of scaled codes take
+constexpr float QT_OPERAND = 9.094947017729282e-13f, QT_OPERAND_BACK = 1099511627776.f;    // 2^-40, 2^40
 
 template <int HD> struct QtSizes {
   static constexpr int KC = HD / 64;                          // tiles of 64 dims
   static constexpr int KS = 2, VS = KC == 1 ? 2 : 1;          // stages of keys and values (shared memory has room for one of values at 128)
   static constexpr int CODES = QT_KEYS * (2 * HD + 8);        // a stage: key codes, value codes, key scales, value scales
-  static constexpr int KEY_DATA = 4 * QT_KEYS * 4;            // a block's u log2(e) scale, e, f, 2^-e of every key; four blocks' worth
-  static constexpr int smem = 1024 + (KC + KS * KC + VS * KC) * QT_TILE + 2 * CODES + 4 * KEY_DATA + (4 + 2) * QT_ROWS * 4 + 256;
+  static constexpr int KEY_DATA = QT_GROUPS * 16 + 4 * QT_KEYS * 4;   // a block's groups {2^k scale log2(e), e, 2^-e, slow}, and of every key (where
+                                                                      // its group is slow) u scale log2(e), e, f 2^-40, 2^-e; four blocks' worth
+  static constexpr int smem = 1024 + (KC + KS * KC + VS * KC) * QT_TILE + 2 * CODES + 4 * KEY_DATA + (2 + 1) * QT_GROUPS * QT_ROWS * 4 + 256;
 };
 
 // Instruction descriptor of kind::f16 with float16 operands: D float32, both K-major, M x N.
@@ -100,8 +106,8 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
   uint8_t* v_s = k_s + KS * KC * QT_TILE;          // [VS][KC][128 keys][128 bytes]
   uint8_t* codes = v_s + VS * KC * QT_TILE;        // [2][CODES]
   uint8_t* key_data = codes + 2 * Z::CODES;        // [4][KEY_DATA]
-  float* row_max = reinterpret_cast<float*>(key_data + 4 * Z::KEY_DATA);      // [block & 1][half of its keys][128 rows]
-  float* row_sum = row_max + 4 * QT_ROWS;          // [half of the keys][128 rows]
+  float* row_max = reinterpret_cast<float*>(key_data + 4 * Z::KEY_DATA);      // [block & 1][group][128 rows]
+  float* row_sum = row_max + 2 * QT_GROUPS * QT_ROWS;      // [group][128 rows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(row_sum + 2 * QT_ROWS);
   uint64_t *q_ready = bars, *c_full = bars + 1, *c_empty = c_full + 2, *k_full = c_empty + 2, *k_empty = k_full + KS, *v_full = k_empty + KS;
   uint64_t *v_empty = v_full + VS, *s_ready = v_empty + VS, *p_ready = s_ready + 2, *o_done = p_ready + 2;
@@ -212,8 +218,8 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
-          for (int s = 0; s < 8; ++s)                                 // 16 keys: 8 columns of the weights of half s / 4
-            umma_f16_ts(tmem + O_COL + c * 64, tmem + b * S_COLS + s / 4 * 64 + s % 4 * 8, (uint32_t)dv + (c * QT_TILE + s * 16 * 128 >> 4), (uint32_t)(dv >> 32), idesc,
+          for (int s = 0; s < 8; ++s)                                 // 16 keys: 8 columns of the weights of group s / 2
+            umma_f16_ts(tmem + O_COL + c * 64, tmem + b * S_COLS + s / 2 * 32 + s % 2 * 8, (uint32_t)dv + (c * QT_TILE + s * 16 * 128 >> 4), (uint32_t)(dv >> 32), idesc,
                         j > 0 || s != 0);
         umma_commit(smem_u32(&o_done[b]));
         umma_commit(smem_u32(&v_empty[st]));
@@ -235,26 +241,56 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       const float* scales = reinterpret_cast<const float*>(codes + cs * Z::CODES + 2 * QT_KEYS * HD) + cw * 32 + lane;
       const bool there = key_of(j) + cw * 32 + lane < n_keys;
       const float u = there ? scales[0] : 0.f, v = there ? scales[QT_KEYS] : 0.f;
-      const bool fine = (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u;
-      const ValueScale vsc = value_scale(fine ? v : 0.f);
-      float* kd = reinterpret_cast<float*>(key_data + (j & 3) * Z::KEY_DATA) + cw * 32 + lane;
-      kd[0] = fine ? u * (a.scale * AQ_LOG2E) : CUDART_NAN_F;
-      kd[QT_KEYS] = vsc.e;
-      kd[2 * QT_KEYS] = vsc.f * QT_OPERAND;
-      kd[3 * QT_KEYS] = vsc.undo;
-#pragma unroll
-      for (int i = 0; i < 32 / ROWS; ++i) {
-        const int r = i * ROWS + sub;
-        const uint4 c = *reinterpret_cast<const uint4*>(src + r * HD + d);
-        uint4 lo, hi;
-        codes_to_half<FMT>(c.x, lo.x, lo.y);
-        codes_to_half<FMT>(c.y, lo.z, lo.w);
-        codes_to_half<FMT>(c.z, hi.x, hi.y);
-        codes_to_half<FMT>(c.w, hi.z, hi.w);
-        uint8_t* dst = k_s + ks * KC * QT_TILE;
-        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d)) = lo;
-        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d + 8)) = hi;
+      // the largest and smallest powers of two of the group's scales; rows that are no number, or as good as zero, have no say
+      const int ub = (int)(__float_as_uint(u) >> 23 & 255u), vb = (int)(__float_as_uint(v) >> 23 & 255u);
+      const bool fine = ub < 255 && vb < 255, counts = there && fine;
+      constexpr int ZERO = 127 - 66;
+      const int umax = __reduce_max_sync(0xffffffffu, counts ? max(ub, 1) : 1), umin = __reduce_min_sync(0xffffffffu, counts && ub > ZERO ? ub : 255);
+      const int vmax = __reduce_max_sync(0xffffffffu, counts ? max(vb, 127 - 60) : 127 - 60), vmin = __reduce_min_sync(0xffffffffu, counts && vb > ZERO ? vb : 255);
+      const bool slow = umax - umin > QT_SPREAD || vmax - vmin > QT_SPREAD;
+      const float un_k = __uint_as_float((uint32_t)(254 - min(umax, 253)) << 23), un_e = __uint_as_float((uint32_t)(254 - min(vmax, 253)) << 23);
+      float* kd = reinterpret_cast<float*>(key_data + (j & 3) * Z::KEY_DATA);
+      if (lane == 0)
+        reinterpret_cast<float4*>(kd)[cw] = make_float4(1.0f / un_k * (a.scale * AQ_LOG2E), (float)(min(vmax, 253) - 127), un_e, slow ? 1.f : 0.f);
+      float mk = fine ? u * un_k : CUDART_NAN_F, mv = fine ? v * un_e : 0.f;
+      if (slow) {
+        const ValueScale vsc = value_scale(fine ? v : 0.f);
+        kd += QT_GROUPS * 4 + cw * 32 + lane;
+        kd[0] = fine ? u * (a.scale * AQ_LOG2E) : CUDART_NAN_F;
+        kd[QT_KEYS] = vsc.e;
+        kd[2 * QT_KEYS] = vsc.f * (QT_OPERAND / AQ_OPERAND);
+        kd[3 * QT_KEYS] = vsc.undo;
+        mk = mv = 1.f;
       }
+      const __half2 hk = __float2half2_rn(mk), hv = __float2half2_rn(mv);
+      const uint32_t fk = *reinterpret_cast<const uint32_t*>(&hk), fv = *reinterpret_cast<const uint32_t*>(&hv);
+      auto tile = [&](const uint8_t* from, uint8_t* to, uint32_t factor, bool values) {
+        uint4 c[32 / ROWS];
+#pragma unroll
+        for (int i = 0; i < 32 / ROWS; ++i) {
+          const int r = i * ROWS + sub;
+          c[i] = *reinterpret_cast<const uint4*>(from + r * HD + d);
+          if (values && key_of(j) + cw * 32 + r >= n_keys) c[i] = make_uint4(0, 0, 0, 0);      // whatever lies there, it meets weights of zero as zero
+        }
+#pragma unroll
+        for (int i = 0; i < 32 / ROWS; ++i) {
+          const int r = i * ROWS + sub;
+          const uint32_t fr = __shfl_sync(0xffffffffu, factor, r);
+          uint32_t w[8];
+          codes_to_half<FMT>(c[i].x, w[0], w[1]);
+          codes_to_half<FMT>(c[i].y, w[2], w[3]);
+          codes_to_half<FMT>(c[i].z, w[4], w[5]);
+          codes_to_half<FMT>(c[i].w, w[6], w[7]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[k]), *reinterpret_cast<const __half2*>(&fr));
+            w[k] = *reinterpret_cast<const uint32_t*>(&x);
+          }
+          *reinterpret_cast<uint4*>(qt_place(to, cw * 32 + r, d)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(qt_place(to, cw * 32 + r, d + 8)) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      };
+      tile(src, k_s + ks * KC * QT_TILE, fk, false);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
@@ -262,20 +298,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
         mbar_arrive(smem_u32(&d_full[j & 3]));
       }
       if (j >= VS && !wait(&v_empty[vs], (j / VS & 1) ^ 1)) break;
-#pragma unroll
-      for (int i = 0; i < 32 / ROWS; ++i) {
-        const int r = i * ROWS + sub;
-        uint4 c = *reinterpret_cast<const uint4*>(src + QT_KEYS * HD + r * HD + d);
-        if (key_of(j) + cw * 32 + r >= n_keys) c = make_uint4(0, 0, 0, 0);      // whatever lies there, it meets weights of zero as zero
-        uint4 lo, hi;
-        codes_to_half<FMT>(c.x, lo.x, lo.y);
-        codes_to_half<FMT>(c.y, lo.z, lo.w);
-        codes_to_half<FMT>(c.z, hi.x, hi.y);
-        codes_to_half<FMT>(c.w, hi.z, hi.w);
-        uint8_t* dst = v_s + vs * KC * QT_TILE;
-        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d)) = lo;
-        *reinterpret_cast<uint4*>(qt_place(dst, cw * 32 + r, d + 8)) = hi;
-      }
+      tile(src + QT_KEYS * HD, v_s + vs * KC * QT_TILE, fv, true);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
@@ -284,87 +307,104 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       }
     }
   } else if (warp >= 8) {
-    const int half = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int part = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // the group of each block, the row
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int rr = row_base + row, tok = rr / g;
     const bool mine = row < rows;
-    // ---- this thread's half of its query row as float16 numbers, lifted by a power of two (exact)
+    auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(quarter + 1) : "memory"); };      // the row's four threads (warps w, w + 4, w + 8, w + 12)
+    auto all_four = [&](const float* at) { return fmaxf(fmaxf(at[row], at[QT_ROWS + row]), fmaxf(at[2 * QT_ROWS + row], at[3 * QT_ROWS + row])); };
+    // ---- this thread's quarter of its query row as float16 numbers, lifted by a power of two (exact)
     float qf;
     {
-      uint4 v[HD / 16];
+      constexpr int N = HD / 32;                   // pieces of eight numbers
+      uint4 v[N];
       uint32_t most = 0;
-      const __nv_bfloat16* src = a.q + (size_t)(tok0 + tok) * a.ldq + (size_t)(kvh * g + rr - tok * g) * HD + half * (HD / 2);
+      const __nv_bfloat16* src = a.q + (size_t)(tok0 + tok) * a.ldq + (size_t)(kvh * g + rr - tok * g) * HD + part * (HD / 4);
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) {
+      for (int i = 0; i < N; ++i) {
         v[i] = mine ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) most = max(most, max(w[k] << 16 & 0x7fffffffu, w[k] & 0x7fff0000u));
       }
-      row_max[half * QT_ROWS + row] = __uint_as_float(most);
-      asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
-      most = max(most, __float_as_uint(row_max[(half ^ 1) * QT_ROWS + row]));
-      asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");      // (both have read, before the maxima are written over)
+      // (magnitudes compare as whole numbers whatever they stand for: kept as such)
+      uint32_t* at = reinterpret_cast<uint32_t*>(row_max);
+      at[part * QT_ROWS + row] = most;
+      meet();
+      most = max(max(at[row], at[QT_ROWS + row]), max(at[2 * QT_ROWS + row], at[3 * QT_ROWS + row]));
+      meet();                                      // (all have read, before the maxima are written over)
       const float lift = query_lift(most);
       qf = 1.0f / lift;
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) {
+      for (int i = 0; i < N; ++i) {
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
         uint32_t h[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) h[k] = aq_pack(__uint_as_float(w[k] << 16) * lift, __uint_as_float(w[k] & 0xffff0000u) * lift);
-        *reinterpret_cast<uint4*>(qt_place(q_s, row, half * (HD / 2) + 8 * i)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(qt_place(q_s, row, part * (HD / 4) + 8 * i)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(q_ready));
     }
-    const uint64_t qf2 = qt_pair(qf, qf);
     const int pos = mine ? pos0 + tok : last_pos;
     float m = -CUDART_INF_F, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < n_blk; ++j) {              // (also behind a wait that ran out: the row's other thread may be at the exchange)
-      const int b = j & 1, key0 = key_of(j) + half * 64;
-      const uint32_t s_addr = tmem + lanes + b * S_COLS + half * 64;
-      const ulonglong2* kd = reinterpret_cast<const ulonglong2*>(key_data + (j & 3) * Z::KEY_DATA) + half * 16;      // four keys' u; 32 further their e, f, 2^-e
+    for (int j = 0; j < n_blk; ++j) {              // (also behind a wait that ran out: the row's other threads may be at the exchange)
+      const int b = j & 1, key0 = key_of(j) + part * 32;
+      const uint32_t s_addr = tmem + lanes + b * S_COLS + part * 32;
+      const float4* gd = reinterpret_cast<const float4*>(key_data + (j & 3) * Z::KEY_DATA);
+      const ulonglong2* kd = reinterpret_cast<const ulonglong2*>(gd + QT_GROUPS) + part * 8;      // (slow) four keys' u; 32 further their e, f, 2^-e
       if (ok) ok = wait(&d_full[j & 3], j >> 2 & 1) && wait(&s_ready[b], j >> 1 & 1);
-      uint64_t x[32];                              // pairs of neighbouring keys
-      float mx = -CUDART_INF_F;
+      float x[32], mx = -CUDART_INF_F;
+      float4 group = make_float4(0.f, 0.f, 0.f, 0.f);
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t r[32];
+        group = gd[part];
+        tmem_ld32(s_addr, reinterpret_cast<uint32_t*>(x));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (group.w == 0.f) {
+          const float f = qf * group.x;
+          const uint64_t f2 = qt_pair(f, f), e2 = qt_pair(group.y, group.y);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {              // a group of 32 keys
-          tmem_ld32(s_addr + c * 32, r);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          for (int i = 0; i < 32; i += 2) {
+            const float2 y = qt_unpair(qt_fma2(qt_pair(x[i], x[i + 1]), f2, e2));
+            x[i] = y.x;
+            x[i + 1] = y.y;
+          }
+        } else {
+          const uint64_t f2 = qt_pair(qf, qf);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const ulonglong2 uu = kd[c * 8 + i], ee = kd[32 + c * 8 + i];
-            x[c * 16 + 2 * i] = qt_fma2(qt_mul2(qt_pair(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), uu.x), qf2, ee.x);
-            x[c * 16 + 2 * i + 1] = qt_fma2(qt_mul2(qt_pair(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), uu.y), qf2, ee.y);
+          for (int i = 0; i < 32; i += 4) {
+            const ulonglong2 u = kd[i / 4], e = kd[32 + i / 4];
+            const float2 y = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i], x[i + 1]), u.x), f2, e.x)), z = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i + 2], x[i + 3]), u.y), f2, e.y));
+            x[i] = y.x;
+            x[i + 1] = y.y;
+            x[i + 2] = z.x;
+            x[i + 3] = z.y;
           }
         }
-        if (key0 + 63 > first_pos || (a.window > 0 && key0 <= last_pos - a.window)) {
-          const int hi = pos - key0, lo = a.window > 0 ? hi - a.window : -1;      // keys lo + 1 .. hi of the thread's 64
+        if (key0 + 31 > first_pos || (a.window > 0 && key0 <= last_pos - a.window)) {
+          const int hi = pos - key0, lo = a.window > 0 ? hi - a.window : -1;      // keys lo + 1 .. hi of the thread's 32
+          uint32_t seen = hi >= 31 ? ~0u : hi < 0 ? 0u : ~(~1u << hi);
+          seen &= lo >= 31 ? 0u : lo < 0 ? ~0u : ~1u << lo;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float2 v = qt_unpair(x[i]);
-            x[i] = qt_pair(2 * i <= hi && 2 * i > lo ? v.x : -CUDART_INF_F, 2 * i + 1 <= hi && 2 * i + 1 > lo ? v.y : -CUDART_INF_F);
-          }
+          for (int i = 0; i < 32; ++i)
+            if (!(seen >> i & 1)) x[i] = -CUDART_INF_F;
         }
         float mx1 = -CUDART_INF_F;
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float2 v = qt_unpair(x[i]), w = qt_unpair(x[i + 1]);
-          mx = fmaxf(mx, fmaxf(v.x, v.y));
-          mx1 = fmaxf(mx1, fmaxf(w.x, w.y));
+        for (int i = 0; i < 32; i += 4) {
+          mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
+          mx1 = fmaxf(mx1, fmaxf(x[i + 2], x[i + 3]));
         }
         mx = fmaxf(mx, mx1);
       }
-      row_max[(b * 2 + half) * QT_ROWS + row] = mx;
-      asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");      // the row's two threads (warps w and w + 4)
+      float* maxima = row_max + b * QT_GROUPS * QT_ROWS;
+      maxima[part * QT_ROWS + row] = mx;
+      meet();
       if (!ok) continue;
-      mx = fmaxf(mx, row_max[(b * 2 + (half ^ 1)) * QT_ROWS + row]);
+      mx = all_four(maxima);
       float rescale = 1.f;
       if (j == 0) {
         m = mx;
@@ -373,14 +413,14 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
         m = mx;
         l *= rescale;
       }
-      if (__any_sync(0xffffffffu, rescale != 1.f)) {       // (rare after the first blocks; both warps of the rows take it)
+      if (__any_sync(0xffffffffu, rescale != 1.f)) {       // (rare after the first blocks; all four warps of the rows take it)
         ok = wait(&o_done[b ^ 1], (j - 1) >> 1 & 1);
         if (!ok) continue;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < HD / 2; c += 8) {
+        for (int c = 0; c < HD / 4; c += 8) {
           uint32_t o[8];
-          const uint32_t o_addr = tmem + lanes + O_COL + half * (HD / 2) + c;
+          const uint32_t o_addr = tmem + lanes + O_COL + part * (HD / 4) + c;
           tmem_ld8(o_addr, o);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
@@ -388,55 +428,70 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
           qt_tmem_st8(o_addr, o);
         }
       }
-      const float ref = m == -CUDART_INF_F ? 0.f : m;
-      const uint64_t bias = qt_pair(AQ_LIFT - ref, AQ_LIFT - ref);
+      const float bias = AQ_LIFT - (m == -CUDART_INF_F ? 0.f : m);
+      const uint64_t bias2 = qt_pair(bias, bias);
       uint64_t sum0 = 0, sum1 = 0;
+      if (group.w == 0.f) {
+        const uint64_t operand2 = qt_pair(QT_OPERAND, QT_OPERAND);
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        uint32_t w[8];
+        for (int i = 0; i < 32; i += 16) {
+          uint32_t w[8];
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {           // four keys
-          const ulonglong2 ff = kd[64 + (i + k) / 2], un = kd[96 + (i + k) / 2];
-          const float2 y0 = qt_unpair(qt_add2(x[i + k], bias)), y1 = qt_unpair(qt_add2(x[i + k + 1], bias));
-          const uint64_t t0 = qt_pair(aq_exp2(y0.x), aq_exp2(y0.y)), t1 = qt_pair(aq_exp2(y1.x), aq_exp2(y1.y));
-          sum0 = qt_fma2(t0, un.x, sum0);
-          sum1 = qt_fma2(t1, un.y, sum1);
-          const float2 p0 = qt_unpair(qt_mul2(t0, ff.x)), p1 = qt_unpair(qt_mul2(t1, ff.y));
-          w[k] = aq_pack(p0.x, p0.y);
-          w[k + 1] = aq_pack(p1.x, p1.y);
+          for (int k = 0; k < 16; k += 2) {
+            const float2 y = qt_unpair(qt_add2(qt_pair(x[i + k], x[i + k + 1]), bias2));
+            const uint64_t t = qt_pair(aq_exp2(y.x), aq_exp2(y.y));
+            if (k & 2) sum1 = qt_add2(sum1, t);
+            else sum0 = qt_add2(sum0, t);
+            const float2 p = qt_unpair(qt_mul2(t, operand2));
+            w[k / 2] = aq_pack(p.x, p.y);
+          }
+          qt_tmem_st8(s_addr + i / 2, w);
         }
-        qt_tmem_st8(s_addr + i, w);
+        const float2 sum = qt_unpair(qt_add2(sum0, sum1));
+        l = fmaf(sum.x + sum.y, group.z, l);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += 16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int k = 0; k < 16; k += 4) {
+            const ulonglong2 f = kd[64 + (i + k) / 4], un = kd[96 + (i + k) / 4];
+            const float2 y = qt_unpair(qt_add2(qt_pair(x[i + k], x[i + k + 1]), bias2)), z = qt_unpair(qt_add2(qt_pair(x[i + k + 2], x[i + k + 3]), bias2));
+            const uint64_t t0 = qt_pair(aq_exp2(y.x), aq_exp2(y.y)), t1 = qt_pair(aq_exp2(z.x), aq_exp2(z.y));
+            sum0 = qt_fma2(t0, un.x, sum0);
+            sum1 = qt_fma2(t1, un.y, sum1);
+            const float2 p0 = qt_unpair(qt_mul2(t0, f.x)), p1 = qt_unpair(qt_mul2(t1, f.y));
+            w[k / 2] = aq_pack(p0.x, p0.y);
+            w[k / 2 + 1] = aq_pack(p1.x, p1.y);
+          }
+          qt_tmem_st8(s_addr + i / 2, w);
+        }
+        const float2 sum = qt_unpair(qt_add2(sum0, sum1));
+        l += sum.x + sum.y;
       }
-      const float2 sum = qt_unpair(qt_add2(sum0, sum1));
-      l += sum.x + sum.y;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&p_ready[b]));
     }
     if (ok) ok = wait(&o_done[(n_blk - 1) & 1], (n_blk - 1) >> 1 & 1);
-    row_sum[half * QT_ROWS + row] = l;
-    asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
-    float inv = QT_OPERAND_BACK / (row_sum[row] + row_sum[QT_ROWS + row]);
+    row_sum[part * QT_ROWS + row] = l;
+    meet();
+    float inv = QT_OPERAND_BACK / ((row_sum[row] + row_sum[QT_ROWS + row]) + (row_sum[2 * QT_ROWS + row] + row_sum[3 * QT_ROWS + row]));
     if (!ok) inv = CUDART_NAN_F;                   // a wait that ran out: nothing that could pass for a result
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    __nv_bfloat16* dst = a.out + (size_t)(tok0 + tok) * a.ldo + (size_t)(kvh * g + rr - tok * g) * HD + half * (HD / 2);
+    __nv_bfloat16* dst = a.out + (size_t)(tok0 + tok) * a.ldo + (size_t)(kvh * g + rr - tok * g) * HD + part * (HD / 4);
 #pragma unroll
-    for (int c = 0; c < HD / 2; c += 32) {
-      uint32_t o[32];
-      tmem_ld32(tmem + lanes + O_COL + half * (HD / 2) + c, o);
+    for (int c = 0; c < HD / 4; c += 8) {
+      uint32_t o[8], h[4];
+      tmem_ld8(tmem + lanes + O_COL + part * (HD / 4) + c, o);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      if (!mine) continue;
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        uint32_t h[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
-          h[k] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-        *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(h[0], h[1], h[2], h[3]);
+      for (int k = 0; k < 4; ++k) {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
+        h[k] = *reinterpret_cast<const uint32_t*>(&y);
       }
+      if (mine) *reinterpret_cast<uint4*>(dst + c) = make_uint4(h[0], h[1], h[2], h[3]);
     }
     __syncwarp();
   }
