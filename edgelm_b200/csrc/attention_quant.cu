@@ -20,11 +20,24 @@ using namespace edgelm;
 // [n_seqs, (nh + 2 nkv) hd]: the kernel rotates, appends the new rows as codes (kcache, vcache, k_scale, v_scale are written) and
 // attends over the cache with them.  Without: `q` holds rotated query heads and the cache every row up to seq_pos.
 // n_splits: blocks that share a sequence's keys, 1 to 16.  Returns 0 or a negative code.
-extern "C" int edgelm_attn_decode_quantized(const void* q, long long ldq, void* out, long long ldo, void* kcache, void* vcache, float* k_scale,
-                                            float* v_scale, int dtype, int format, const int32_t* page_table, int table_stride, int n_pages,
-                                            const int32_t* seq_slot, const int32_t* seq_pos, const float* cos_t, const float* sin_t, int max_pos,
-                                            int n_seqs, int nh, int nkv, int hd, float scale, int n_splits, int window, int meta_ready, int* err,
-                                            cudaStream_t stream) {
+// (Arguments as one struct, 8-byte fields first: see quant_cache.cu.)
+struct QuantDecodeCall {
+  const void* q;
+  void* out;
+  void *kcache, *vcache;
+  float *k_scale, *v_scale;
+  const int32_t *page_table, *seq_slot, *seq_pos;
+  const float *cos_t, *sin_t;
+  int* err;
+  cudaStream_t stream;
+  long long ldq, ldo;
+  int dtype, format, table_stride, n_pages, max_pos, n_seqs, nh, nkv, hd, n_splits, window, meta_ready;
+  float scale;
+};
+
+extern "C" int edgelm_attn_decode_quantized(const QuantDecodeCall* call) {
+  const auto [q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos_t, sin_t, err, stream, ldq, ldo, dtype, format, table_stride, n_pages,
+              max_pos, n_seqs, nh, nkv, hd, n_splits, window, meta_ready, scale] = *call;
   if (n_seqs == 0) return 0;
   const char* who = "attn_decode_quantized";
   EL_REFUSE(nh > 0 && nkv > 0 && nh % nkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, nh, nkv);
@@ -52,11 +65,22 @@ extern "C" int edgelm_attn_decode_quantized(const void* q, long long ldq, void* 
 
 // New tokens, any number a sequence, as tiles of at most `max_tile_tokens` (up to 128) consecutive tokens of one sequence; their keys and
 // values are in the cache already.  n_splits: blocks that share a row tile's keys, 1 to 8 (mma.sync).  form: 0 by sizes, 1 mma.sync, 2 tcgen05.
-extern "C" int edgelm_attn_prefill_quantized(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache,
-                                             const float* k_scale, const float* v_scale, int dtype, int format, const int32_t* page_table,
-                                             int table_stride, int n_pages, const int32_t* seq_slot, const int32_t* tile_seq, const int32_t* tile_tok0,
-                                             const int32_t* tile_ntok, const int32_t* tile_pos0, int n_tiles, int max_tile_tokens, int nh, int nkv,
-                                             int hd, float scale, int n_splits, int window, int form, int* err, cudaStream_t stream) {
+struct QuantPrefillCall {
+  const void* q;
+  void* out;
+  const void *kcache, *vcache;
+  const float *k_scale, *v_scale;
+  const int32_t *page_table, *seq_slot, *tile_seq, *tile_tok0, *tile_ntok, *tile_pos0;
+  int* err;
+  cudaStream_t stream;
+  long long ldq, ldo;
+  int dtype, format, table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, n_splits, window, form;
+  float scale;
+};
+
+extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
+  const auto [q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok, tile_pos0, err, stream, ldq, ldo, dtype, format,
+              table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, n_splits, window, form, scale] = *call;
   if (n_tiles == 0) return 0;
   const char* who = "attn_prefill_quantized";
   EL_REFUSE(nh > 0 && nkv > 0 && nh % nkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, nh, nkv);

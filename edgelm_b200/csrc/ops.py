@@ -8,6 +8,7 @@ raises.
 """
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -1552,17 +1553,25 @@ QUANT_MAX_SPLITS = 16      # blocks that share a sequence's keys in its decode a
 _QUANT_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
-def _entry(name, kinds):
-    """The library's function `name`, taking Python numbers: a letter an argument (p pointer, i int, l long long, f float)."""
-    fn = getattr(lib(), name)
+# The library's functions of the 8-bit cache take one struct, laid out as in quant_cache.cu and attention_quant.cu (Q: pointers and pitches).
+_QUANT_APPEND = struct.Struct("@14Q9i").pack
+_QUANT_ROWS = struct.Struct("@12Q7i").pack
+_QUANT_DECODE = struct.Struct("@13Q2q12if").pack
+_QUANT_PREFILL = struct.Struct("@14Q2q12if").pack
+
+
+def _call_packed(name, packed, launches):
+    fn = getattr(_lib or lib(), name)
     if fn.argtypes is None:
-        fn.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}[k] for k in kinds]
-    return fn
+        fn.argtypes = [ctypes.c_char_p]
+    if fn(packed):
+        raise KernelError(lib().edgelm_last_error().decode())
+    count_launches(launches)
 
 
 def _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what):
-    """Checks the cache's tensors; the format's code and the device's index.  (Messages are made only when something is wrong: these
-    calls are made once a layer and token.)"""
+    """Checks the cache's tensors; the format's code, the device's index and the number of pages.  (Messages are made only when something
+    is wrong: these calls are made once a layer and token.)"""
     code = _QUANT_CODES.get(kcache.dtype)
     if code is None or vcache.dtype != kcache.dtype:
         raise KernelError(f"{what}: the cache's codes must be int8 or float8_e4m3fn, keys and values alike")
@@ -1575,24 +1584,30 @@ def _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what):
     if not (kcache.is_contiguous() and vcache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise KernelError(f"{what}: the cache must be contiguous")
     device = kcache.get_device()
-    if device < 0 or device != torch.cuda.current_device() or not device == vcache.get_device() == k_scale.get_device() == v_scale.get_device():
+    if device < 0 or device != torch._C._cuda_getDevice() or not device == vcache.get_device() == k_scale.get_device() == v_scale.get_device():
         raise KernelError(f"{what}: the cache must lie on the current device")
-    return code, device
+    return code, device, shape[0]
 
 
 def _quant_steps(page_table, tensors, device, what):
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.get_device() != device or page_table.stride(1) != 1:
+    """Checks the page table and the (tensor, least count) pairs; the table's pitch."""
+    stride = page_table.stride()
+    if len(stride) != 2 or stride[1] != 1 or page_table.dtype != torch.int32 or page_table.get_device() != device:
         raise KernelError(f"{what}: the page table must be int32 rows on the cache's device")
     for t, n in tensors:
         if t.dtype != torch.int32 or t.get_device() != device or not t.is_contiguous() or t.numel() < n:
             raise KernelError(f"{what}: positions, indices, tiles and the error word must be contiguous int32 tensors on the cache's device, one number each "
                               f"per token, sequence or tile (at least {n} here)")
+    return stride[0]
 
 
 def _quant_tables(cos, sin, hd, device, what):
-    if not (cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == hd // 2 and
+    """Checks the position tables; how many positions they have."""
+    shape = cos.shape
+    if not (cos.dtype == sin.dtype == torch.float32 and sin.shape == shape and len(shape) == 2 and shape[1] == hd // 2 and
             cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == device):
         raise KernelError(f"{what}: the position tables must be float32 [positions, {hd // 2}] on the cache's device")
+    return shape[0]
 
 
 def _heads(nh, nkv, hd, what):
@@ -1603,14 +1618,16 @@ def _heads(nh, nkv, hd, what):
 
 
 def _quant_rows(q, out, width, nh, hd, device, what):
-    if q.dtype != out.dtype or q.dim() != 2 or out.dim() != 2 or q.stride(1) != 1 or out.stride(1) != 1:
+    """Checks rows of queries and outputs; their pitches and counts."""
+    (qs, os), (q_shape, o_shape) = (q.stride(), out.stride()), (q.shape, out.shape)
+    if q.dtype != out.dtype or len(qs) != 2 or len(os) != 2 or qs[1] != 1 or os[1] != 1:
         raise KernelError(f"{what}: queries and outputs must be rows of one type")
-    if q.shape[1] < width or out.shape[1] < nh * hd or q.get_device() != device or out.get_device() != device:
+    if q_shape[1] < width or o_shape[1] < nh * hd or q.get_device() != device or out.get_device() != device:
         raise KernelError(f"{what}: rows of {width} and {nh * hd} numbers on the cache's device are wanted")
+    return qs[0], os[0], q_shape[0], o_shape[0]
 
 
-def _raw_stream(device):
-    return torch._C._cuda_getCurrentRawStream(device)
+_raw_stream = torch._C._cuda_getCurrentRawStream     # a device's index -> the current stream's handle
 
 
 def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, kcache, vcache, k_scale, v_scale, nh, nkv, hd, err, q_out=None):
@@ -1618,36 +1635,37 @@ def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, 
     [tokens, nh * hd] where given: `qkv` is then left as it was), write k and v as codes and scales into their pages."""
     what = "rope_quantize_append"
     _heads(nh, nkv, hd, what)
-    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
-    if not qkv.is_contiguous() or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd or qkv.get_device() != device:
+    code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    shape = qkv.shape
+    if not qkv.is_contiguous() or len(shape) != 2 or shape[1] != (nh + 2 * nkv) * hd or qkv.get_device() != device:
         raise KernelError(f"{what}: the projections must be contiguous rows of {(nh + 2 * nkv) * hd} numbers on the cache's device")
-    T = qkv.shape[0]
+    T = shape[0]
     if q_out is not None and (q_out.shape != (T, nh * hd) or q_out.dtype != qkv.dtype or not q_out.is_contiguous() or q_out.get_device() != device):
         raise KernelError(f"{what}: q_out must be contiguous rows of {nh * hd} numbers, one per token, of the projections' type")
-    _quant_tables(cos, sin, hd, device, what)
-    _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
-    _check(_entry("edgelm_rope_quantize_append", "ppiipppp" "iippi" "pppp" "iiiipp")(
-        qkv.data_ptr(), q_out.data_ptr() if q_out is not None else None, _dt(qkv), code, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-        kcache.shape[0], cos.data_ptr(), sin.data_ptr(), cos.shape[0], kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-        T, nh, nkv, hd, err.data_ptr(), _raw_stream(device)), launches=1 if T else 0)
+    max_pos = _quant_tables(cos, sin, hd, device, what)
+    pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
+    _call_packed("edgelm_rope_quantize_append", _QUANT_APPEND(
+        qkv.data_ptr(), q_out.data_ptr() if q_out is not None else 0, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(),
+        cos.data_ptr(), sin.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), err.data_ptr(), _raw_stream(device),
+        _dt(qkv), code, pitch, n_pages, max_pos, T, nh, nkv, hd), 1 if T else 0)
 
 
 def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot, page_table, keys, values, err):
     """keys[t], values[t] = what the 8-bit cache holds for token t (position tok_pos[t] of sequence tok_seq[t]): [T, kv_heads, head_dim],
     float32 or bfloat16, code * scale in float32 rounded once.  A token whose page the cache does not have: zeros, and a bit of `err`."""
     what = "quantized_rows"
-    if keys.dim() != 3 or keys.shape != values.shape or keys.dtype != values.dtype or not (keys.is_contiguous() and values.is_contiguous()):
+    shape = keys.shape
+    if len(shape) != 3 or shape != values.shape or keys.dtype != values.dtype or not (keys.is_contiguous() and values.is_contiguous()):
         raise KernelError(f"{what}: rows must be contiguous [tokens, kv_heads, head_dim], keys and values alike")
-    T, nkv, hd = keys.shape
+    T, nkv, hd = shape
     _heads(nkv, nkv, hd, what)
-    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
     if not keys.get_device() == values.get_device() == device:
         raise KernelError(f"{what}: rows must lie on the cache's device")
-    _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
-    _check(_entry("edgelm_quantized_rows", "ppppi" "ppppii" "ppi" "iiipp")(
-        kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), code, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(),
-        page_table.data_ptr(), page_table.stride(0), kcache.shape[0], keys.data_ptr(), values.data_ptr(), _dt(keys), T, nkv, hd, err.data_ptr(),
-        _raw_stream(device)), launches=1 if T else 0)
+    pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
+    _call_packed("edgelm_quantized_rows", _QUANT_ROWS(
+        kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(),
+        page_table.data_ptr(), keys.data_ptr(), values.data_ptr(), err.data_ptr(), _raw_stream(device), code, _dt(keys), pitch, n_pages, T, nkv, hd), 1 if T else 0)
 
 
 def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
@@ -1664,24 +1682,23 @@ def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
 def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv, hd, scale, n_splits,
                            err, window, meta_ready):
     _heads(nh, nkv, hd, what)
-    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
-    _quant_rows(q, out, nh * hd if cos is None else (nh + 2 * nkv) * hd, nh, hd, device, what)
-    if n_seqs < 0 or q.shape[0] < n_seqs or out.shape[0] < n_seqs:
+    code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    ldq, ldo, rows_q, rows_out = _quant_rows(q, out, nh * hd if cos is None else (nh + 2 * nkv) * hd, nh, hd, device, what)
+    if n_seqs < 0 or rows_q < n_seqs or rows_out < n_seqs:
         raise KernelError(f"{what}: a row of queries and of outputs per sequence is wanted")
-    _quant_steps(page_table, ((seq_slot, n_seqs), (seq_pos, n_seqs)) + (((err, 1),) if err is not None else ()), device, what)
+    pitch = _quant_steps(page_table, ((seq_slot, n_seqs), (seq_pos, n_seqs)) if err is None else ((seq_slot, n_seqs), (seq_pos, n_seqs), (err, 1)), device, what)
     window = int(window or 0)
     if n_splits is None:
         keys = page_table.shape[1] * PAGE
         n_splits = quantized_decode_splits(n_seqs, nh, nkv, hd, min(keys, window) if window > 0 else keys)
-    cos_ptr = sin_ptr = None
-    max_pos = 0
+    cos_ptr = sin_ptr = max_pos = 0
     if cos is not None:
-        _quant_tables(cos, sin, hd, device, what)
-        cos_ptr, sin_ptr, max_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    _check(_entry("edgelm_attn_decode_quantized", "plplpppp" "iipiipp" "ppi" "iiiif" "iiipp")(
-        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _dt(q), code,
-        page_table.data_ptr(), page_table.stride(0), kcache.shape[0], seq_slot.data_ptr(), seq_pos.data_ptr(), cos_ptr, sin_ptr, max_pos, n_seqs, nh, nkv,
-        hd, scale, n_splits, window, 1 if meta_ready else 0, err.data_ptr() if err is not None else None, _raw_stream(device)), launches=1 if n_seqs else 0)
+        max_pos = _quant_tables(cos, sin, hd, device, what)
+        cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
+    _call_packed("edgelm_attn_decode_quantized", _QUANT_DECODE(
+        q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
+        seq_pos.data_ptr(), cos_ptr, sin_ptr, err.data_ptr() if err is not None else 0, _raw_stream(device), ldq, ldo, _dt(q), code, pitch, n_pages, max_pos,
+        n_seqs, nh, nkv, hd, n_splits, window, 1 if meta_ready else 0, scale), 1 if n_seqs else 0)
 
 
 def attn_decode_quantized(q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, n_seqs, nh, nkv, hd, scale, n_splits=None,
@@ -1720,19 +1737,18 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     `form`: 0 by sizes, 1 on mma.sync, 2 on tcgen05 (bfloat16, head size 64 or 128, with the error word)."""
     what = "attn_prefill_quantized"
     _heads(nh, nkv, hd, what)
-    code, device = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
-    _quant_rows(qkv, out, nh * hd, nh, hd, device, what)
-    if qkv.shape[0] != out.shape[0]:
+    code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
+    ldq, ldo, rows_q, rows_out = _quant_rows(qkv, out, nh * hd, nh, hd, device, what)
+    if rows_q != rows_out:
         raise KernelError(f"{what}: a row of outputs per row of queries is wanted")
-    _quant_steps(page_table, ((seq_slot, 0), (tile_seq, n_tiles), (tile_tok0, n_tiles), (tile_ntok, n_tiles), (tile_pos0, n_tiles)) +
-                 (((err, 1),) if err is not None else ()), device, what)
+    wanted = ((seq_slot, 0), (tile_seq, n_tiles), (tile_tok0, n_tiles), (tile_ntok, n_tiles), (tile_pos0, n_tiles))
+    pitch = _quant_steps(page_table, wanted if err is None else wanted + ((err, 1),), device, what)
     window = int(window or 0)
-    most = max(1, min(QUANT_PREFILL_TILE, qkv.shape[0]))
+    most = max(1, min(QUANT_PREFILL_TILE, rows_q))
     if n_splits is None:
         keys = max_keys or page_table.shape[1] * PAGE
         n_splits = quantized_prefill_splits(nkv * n_tiles * -(-most * (nh // nkv) // 64), hd, min(keys, window + most) if window > 0 else keys)
-    _check(_entry("edgelm_attn_prefill_quantized", "plplpppp" "iipii" "ppppp" "iiiii" "fiiipp")(
-        qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _dt(qkv),
-        code, page_table.data_ptr(), page_table.stride(0), kcache.shape[0], seq_slot.data_ptr(), tile_seq.data_ptr(), tile_tok0.data_ptr(),
-        tile_ntok.data_ptr(), tile_pos0.data_ptr(), n_tiles, most, nh, nkv, hd, scale, n_splits, window, form, err.data_ptr() if err is not None else None,
-        _raw_stream(device)), launches=1 if n_tiles else 0)
+    _call_packed("edgelm_attn_prefill_quantized", _QUANT_PREFILL(
+        qkv.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
+        tile_seq.data_ptr(), tile_tok0.data_ptr(), tile_ntok.data_ptr(), tile_pos0.data_ptr(), err.data_ptr() if err is not None else 0, _raw_stream(device),
+        ldq, ldo, _dt(qkv), code, pitch, n_pages, n_tiles, most, nh, nkv, hd, n_splits, window, form, scale), 1 if n_tiles else 0)

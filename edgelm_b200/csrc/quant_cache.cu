@@ -227,51 +227,70 @@ static void launch_append(const void* qkv, void* q_out, const int32_t* tok_pos, 
 
 using namespace edgelm;
 
-// q_out: rows [n_tokens, nh hd] for the rotated queries, or null: back in place.
-extern "C" int edgelm_rope_quantize_append(void* qkv, void* q_out, int dtype, int format, const int32_t* tok_pos, const int32_t* tok_seq, const int32_t* seq_slot,
-                                           const int32_t* page_table, int table_stride, int n_pages, const float* cos_t, const float* sin_t,
-                                           int max_pos, void* kcache, void* vcache, float* k_scale, float* v_scale, int n_tokens, int nh, int nkv,
-                                           int hd, int* err, cudaStream_t stream) {
-  if (n_tokens == 0) return 0;
-  EL_REFUSE(n_tokens > 0 && nh > 0 && nkv > 0, "rope_quantize_append: bad sizes");
-  EL_REFUSE(hd >= 16 && hd <= 256 && hd % 16 == 0, "rope_quantize_append: head size %d (takes 16..256 in steps of 16)", hd);
-  EL_REFUSE((format == QF_INT8 || format == QF_FP8) && (dtype == DT_F32 || dtype == DT_BF16), "rope_quantize_append: format %d, dtype %d", format, dtype);
-  EL_REFUSE((uintptr_t)qkv % 16 == 0 && (uintptr_t)q_out % 16 == 0 && (uintptr_t)cos_t % 16 == 0 && (uintptr_t)sin_t % 16 == 0 && (uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0,
+// The entry points of the 8-bit cache take their arguments as one struct: their callers make a call a layer and token, and packing a struct
+// takes a sixth of the time that converting thirty arguments one by one does (0.4 against 1.9 us in Python).  8-byte fields first.
+struct QuantAppendCall {
+  void *qkv, *q_out;                                        // q_out: rows [n_tokens, nh hd] for the rotated queries, or null: back in place
+  const int32_t *tok_pos, *tok_seq, *seq_slot, *page_table;
+  const float *cos_t, *sin_t;
+  void *kcache, *vcache;
+  float *k_scale, *v_scale;
+  int* err;
+  cudaStream_t stream;
+  int dtype, format, table_stride, n_pages, max_pos, n_tokens, nh, nkv, hd;
+};
+
+extern "C" int edgelm_rope_quantize_append(const QuantAppendCall* call) {
+  const QuantAppendCall& c = *call;
+  if (c.n_tokens == 0) return 0;
+  EL_REFUSE(c.n_tokens > 0 && c.nh > 0 && c.nkv > 0, "rope_quantize_append: bad sizes");
+  EL_REFUSE(c.hd >= 16 && c.hd <= 256 && c.hd % 16 == 0, "rope_quantize_append: head size %d (takes 16..256 in steps of 16)", c.hd);
+  EL_REFUSE((c.format == QF_INT8 || c.format == QF_FP8) && (c.dtype == DT_F32 || c.dtype == DT_BF16), "rope_quantize_append: format %d, dtype %d", c.format, c.dtype);
+  EL_REFUSE((uintptr_t)c.qkv % 16 == 0 && (uintptr_t)c.q_out % 16 == 0 && (uintptr_t)c.cos_t % 16 == 0 && (uintptr_t)c.sin_t % 16 == 0 &&
+                (uintptr_t)c.kcache % 16 == 0 && (uintptr_t)c.vcache % 16 == 0,
             "rope_quantize_append: rows must start on 16-byte boundaries");
-  EL_REFUSE((long long)n_tokens * (nh + 2 * nkv) < 0x7fffffffLL, "rope_quantize_append: grid too large");
-  auto go = [&](auto fn) { fn(qkv, q_out, tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, cos_t, sin_t, max_pos, kcache, vcache, k_scale, v_scale,
-                              n_tokens, nh, nkv, hd, err, stream); };
-  if (dtype == DT_F32) format == QF_INT8 ? go(launch_append<float, QF_INT8>) : go(launch_append<float, QF_FP8>);
-  else format == QF_INT8 ? go(launch_append<__nv_bfloat16, QF_INT8>) : go(launch_append<__nv_bfloat16, QF_FP8>);
+  EL_REFUSE((long long)c.n_tokens * (c.nh + 2 * c.nkv) < 0x7fffffffLL, "rope_quantize_append: grid too large");
+  auto go = [&](auto fn) { fn(c.qkv, c.q_out, c.tok_pos, c.tok_seq, c.seq_slot, c.page_table, c.table_stride, c.n_pages, c.cos_t, c.sin_t, c.max_pos, c.kcache,
+                              c.vcache, c.k_scale, c.v_scale, c.n_tokens, c.nh, c.nkv, c.hd, c.err, c.stream); };
+  if (c.dtype == DT_F32) c.format == QF_INT8 ? go(launch_append<float, QF_INT8>) : go(launch_append<float, QF_FP8>);
+  else c.format == QF_INT8 ? go(launch_append<__nv_bfloat16, QF_INT8>) : go(launch_append<__nv_bfloat16, QF_FP8>);
   EL_LAUNCH_CHECK("rope_quantize_append");
   return 0;
 }
 
-extern "C" int edgelm_quantized_rows(const void* kcache, const void* vcache, const float* k_scale, const float* v_scale, int format,
-                                     const int32_t* tok_pos, const int32_t* tok_seq, const int32_t* seq_slot, const int32_t* page_table,
-                                     int table_stride, int n_pages, void* keys, void* values, int dtype, int n_tokens, int nkv, int hd, int* err,
-                                     cudaStream_t stream) {
-  if (n_tokens == 0) return 0;
-  EL_REFUSE(n_tokens > 0 && nkv > 0, "quantized_rows: bad sizes");
-  EL_REFUSE(hd >= 16 && hd <= 256 && hd % 16 == 0, "quantized_rows: head size %d (takes 16..256 in steps of 16)", hd);
-  EL_REFUSE((format == QF_INT8 || format == QF_FP8) && (dtype == DT_F32 || dtype == DT_BF16), "quantized_rows: format %d, dtype %d", format, dtype);
-  EL_REFUSE((uintptr_t)keys % 16 == 0 && (uintptr_t)values % 16 == 0 && (uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0,
+struct QuantRowsCall {
+  const void *kcache, *vcache;
+  const float *k_scale, *v_scale;
+  const int32_t *tok_pos, *tok_seq, *seq_slot, *page_table;
+  void *keys, *values;
+  int* err;
+  cudaStream_t stream;
+  int format, dtype, table_stride, n_pages, n_tokens, nkv, hd;
+};
+
+extern "C" int edgelm_quantized_rows(const QuantRowsCall* call) {
+  const QuantRowsCall& c = *call;
+  if (c.n_tokens == 0) return 0;
+  EL_REFUSE(c.n_tokens > 0 && c.nkv > 0, "quantized_rows: bad sizes");
+  EL_REFUSE(c.hd >= 16 && c.hd <= 256 && c.hd % 16 == 0, "quantized_rows: head size %d (takes 16..256 in steps of 16)", c.hd);
+  EL_REFUSE((c.format == QF_INT8 || c.format == QF_FP8) && (c.dtype == DT_F32 || c.dtype == DT_BF16), "quantized_rows: format %d, dtype %d", c.format, c.dtype);
+  EL_REFUSE((uintptr_t)c.keys % 16 == 0 && (uintptr_t)c.values % 16 == 0 && (uintptr_t)c.kcache % 16 == 0 && (uintptr_t)c.vcache % 16 == 0,
             "quantized_rows: rows must start on 16-byte boundaries");
-  EL_REFUSE((long long)n_tokens * 2 * nkv < 0x7fffffffLL, "quantized_rows: grid too large");
-  const bool many = n_tokens >= QA_MANY_TOKENS;
-  const int per_warp = 32 * (many ? QA_MANY_PIECES : 1), warps = (2 * nkv * (hd / 16) + per_warp - 1) / per_warp;
-  const dim3 grid((unsigned)(((long long)n_tokens * warps + QA_THREADS / 32 - 1) / (QA_THREADS / 32)));
+  EL_REFUSE((long long)c.n_tokens * 2 * c.nkv < 0x7fffffffLL, "quantized_rows: grid too large");
+  const bool many = c.n_tokens >= QA_MANY_TOKENS;
+  const int per_warp = 32 * (many ? QA_MANY_PIECES : 1), warps = (2 * c.nkv * (c.hd / 16) + per_warp - 1) / per_warp;
+  const dim3 grid((unsigned)(((long long)c.n_tokens * warps + QA_THREADS / 32 - 1) / (QA_THREADS / 32)));
   auto go = [&](auto kern, auto* out) {
     using T = std::remove_pointer_t<decltype(out)>;
-    launch_pdl(pdl_bit_for_tokens(n_tokens), kern, grid, dim3(QA_THREADS), (size_t)0, stream, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale,
-               tok_pos, tok_seq, seq_slot, page_table, table_stride, n_pages, (T*)keys, (T*)values, n_tokens, nkv, hd, warps, err);
+    launch_pdl(pdl_bit_for_tokens(c.n_tokens), kern, grid, dim3(QA_THREADS), (size_t)0, c.stream, (const uint8_t*)c.kcache, (const uint8_t*)c.vcache, c.k_scale,
+               c.v_scale, c.tok_pos, c.tok_seq, c.seq_slot, c.page_table, c.table_stride, c.n_pages, (T*)c.keys, (T*)c.values, c.n_tokens, c.nkv, c.hd, warps, c.err);
   };
   auto type = [&](auto* out) {
     using T = std::remove_pointer_t<decltype(out)>;
-    if (format == QF_INT8) many ? go(quantized_rows_kernel<T, QF_INT8, QA_MANY_PIECES>, out) : go(quantized_rows_kernel<T, QF_INT8, 1>, out);
+    if (c.format == QF_INT8) many ? go(quantized_rows_kernel<T, QF_INT8, QA_MANY_PIECES>, out) : go(quantized_rows_kernel<T, QF_INT8, 1>, out);
     else many ? go(quantized_rows_kernel<T, QF_FP8, QA_MANY_PIECES>, out) : go(quantized_rows_kernel<T, QF_FP8, 1>, out);
   };
-  if (dtype == DT_F32) type((float*)nullptr);
+  if (c.dtype == DT_F32) type((float*)nullptr);
   else type((__nv_bfloat16*)nullptr);
   EL_LAUNCH_CHECK("quantized_rows");
   return 0;

@@ -1,4 +1,6 @@
 """What the 8-bit cache's entry points refuse, before anything is launched (no device is needed)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -67,19 +69,37 @@ def test_heads_that_do_not_divide(which):
 def test_the_library_refuses_too():
     lib = ops.lib()
     message = lambda: lib.edgelm_last_error().decode()      # noqa: E731
-    decode = ops._entry("edgelm_attn_decode_quantized", "plplpppp" "iipiipp" "ppi" "iiiif" "iiipp")
 
-    def go(dtype=0, fmt=0, n_seqs=1, nh=4, nkv=2, hd=64, splits=1, window=0, cos=None, sin=None, max_pos=0, k=256):
-        return decode(256, 512, 256, 512, k, 256, 256, 256, dtype, fmt, 256, 1, 1, 256, 256, cos, sin, max_pos, n_seqs, nh, nkv, hd, 0.1, splits, window, 0, None, None)
+    def run(name, packed):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.c_char_p]
+        return fn(packed)
+
+    def go(dtype=0, fmt=0, n_seqs=1, nh=4, nkv=2, hd=64, splits=1, window=0, cos=0, sin=0, max_pos=0, k=256):
+        return run("edgelm_attn_decode_quantized", ops._QUANT_DECODE(256, 256, k, 256, 256, 256, 256, 256, 256, cos, sin, 0, 0, 512, 512, dtype, fmt, 1, 1, max_pos,
+                                                                     n_seqs, nh, nkv, hd, splits, window, 0, 0.1))
     assert go(n_seqs=0) == 0
     for bad, word in (({"nh": 3}, "multiple"), ({"hd": 20}, "head size"), ({"fmt": 2}, "format"), ({"dtype": 5}, "dtype"), ({"splits": 17}, "splits"),
                       ({"splits": 0}, "splits"), ({"window": -1}, "window"), ({"cos": 256}, "tables"), ({"n_seqs": 70000}, "sequences"), ({"k": 264}, "16-byte")):
         assert go(**bad) < 0 and word in message(), (bad, message())
-    prefill = ops._entry("edgelm_attn_prefill_quantized", "plplpppp" "iipii" "ppppp" "iiiii" "fiiipp")
 
     def go2(dtype=0, fmt=0, n_tiles=1, most=128, nh=4, nkv=2, hd=64, splits=1, window=0, q=256, ldq=512, form=0):
-        return prefill(q, ldq, 256, 512, 256, 256, 256, 256, dtype, fmt, 256, 1, 1, 256, 256, 256, 256, 256, n_tiles, most, nh, nkv, hd, 0.1, splits, window, form, None, None)
+        return run("edgelm_attn_prefill_quantized", ops._QUANT_PREFILL(q, 256, 256, 256, 256, 256, 256, 256, 256, 256, 256, 256, 0, 0, ldq, 512, dtype, fmt, 1, 1, n_tiles,
+                                                                       most, nh, nkv, hd, splits, window, form, 0.1))
     assert go2(n_tiles=0) == 0
     for bad, word in (({"nh": 3}, "multiple"), ({"hd": 20}, "head size"), ({"fmt": 2}, "format"), ({"most": 129}, "tokens"), ({"splits": 9}, "splits"),
-                      ({"window": -1}, "window"), ({"form": 3}, "form"), ({"form": 2}, "tcgen05"), ({"q": 264}, "16-byte"), ({"ldq": 510}, "multiple of 4"), ({"n_tiles": 60000, "nh": 8}, "65,535")):
+                      ({"window": -1}, "window"), ({"form": 3}, "form"), ({"form": 2}, "tcgen05"), ({"q": 264}, "16-byte"), ({"ldq": 510}, "multiple of 4"),
+                      ({"n_tiles": 60000, "nh": 8}, "65,535")):
         assert go2(**bad) < 0 and word in message(), (bad, message())
+
+    def go3(n=1, nh=4, hd=64, fmt=0, dtype=0, qkv=256):
+        return run("edgelm_rope_quantize_append", ops._QUANT_APPEND(qkv, 0, 256, 256, 256, 256, 256, 256, 256, 256, 256, 256, 256, 0, dtype, fmt, 1, 1, 8, n, nh, 2, hd))
+    assert go3(n=0) == 0
+    for bad, word in (({"nh": 0}, "sizes"), ({"hd": 40}, "head size"), ({"fmt": 3}, "format"), ({"dtype": 2}, "dtype"), ({"qkv": 260}, "16-byte"), ({"n": 1 << 30}, "grid")):
+        assert go3(**bad) < 0 and word in message(), (bad, message())
+
+    def go4(n=1, nkv=2, hd=64, fmt=0, dtype=0, keys=256):
+        return run("edgelm_quantized_rows", ops._QUANT_ROWS(256, 256, 256, 256, 256, 256, 256, 256, keys, 256, 256, 0, fmt, dtype, 1, 1, n, nkv, hd))
+    assert go4(n=0) == 0
+    for bad, word in (({"nkv": 0}, "sizes"), ({"hd": 40}, "head size"), ({"fmt": 3}, "format"), ({"dtype": 2}, "dtype"), ({"keys": 260}, "16-byte"), ({"n": 1 << 30}, "grid")):
+        assert go4(**bad) < 0 and word in message(), (bad, message())
