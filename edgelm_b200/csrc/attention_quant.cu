@@ -19,7 +19,8 @@ using namespace edgelm;
 // One new token a sequence.  With the position tables (cos_t, sin_t [max_pos, hd / 2]) `q` holds the raw q, k, v projections
 // [n_seqs, (nh + 2 nkv) hd]: the kernel rotates, appends the new rows as codes (kcache, vcache, k_scale, v_scale are written) and
 // attends over the cache with them.  Without: `q` holds rotated query heads and the cache every row up to seq_pos.
-// n_splits: blocks that share a sequence's keys, 1 to 16.  Returns 0 or a negative code.
+// n_splits: blocks that share a sequence's keys, 1 to 8 or a multiple of 8 up to 128; from 16 on `part` is scratch for n_seqs nh (n_splits / 8)
+// (hd + 2) floats.  Returns 0 or a negative code.
 // (Arguments as one struct, 8-byte fields first: see quant_cache.cu.)
 struct QuantDecodeCall {
   const void* q;
@@ -29,6 +30,7 @@ struct QuantDecodeCall {
   const int32_t *page_table, *seq_slot, *seq_pos;
   const float *cos_t, *sin_t;
   int* err;
+  float* part;
   cudaStream_t stream;
   long long ldq, ldo;
   int dtype, format, table_stride, n_pages, max_pos, n_seqs, nh, nkv, hd, n_splits, window, meta_ready;
@@ -36,7 +38,7 @@ struct QuantDecodeCall {
 };
 
 extern "C" int edgelm_attn_decode_quantized(const QuantDecodeCall* call) {
-  const auto [q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos_t, sin_t, err, stream, ldq, ldo, dtype, format, table_stride, n_pages,
+  const auto [q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos_t, sin_t, err, part, stream, ldq, ldo, dtype, format, table_stride, n_pages,
               max_pos, n_seqs, nh, nkv, hd, n_splits, window, meta_ready, scale] = *call;
   if (n_seqs == 0) return 0;
   const char* who = "attn_decode_quantized";
@@ -46,16 +48,23 @@ extern "C" int edgelm_attn_decode_quantized(const QuantDecodeCall* call) {
   EL_REFUSE(n_seqs > 0 && n_seqs <= 65535, "%s: %d sequences (takes up to 65,535)", who, n_seqs);
   const int chunks = (nh / nkv + QD_HEADS - 1) / QD_HEADS;
   EL_REFUSE((long long)nkv * chunks <= 65535, "%s: too many heads", who);
-  EL_REFUSE(n_splits >= 1 && n_splits <= QD_MAX_SPLITS, "%s: %d splits (takes 1 to %d)", who, n_splits, QD_MAX_SPLITS);
+  EL_REFUSE(n_splits >= 1 && n_splits <= QD_CLUSTER * QD_MAX_GROUPS && (n_splits <= QD_CLUSTER || n_splits % QD_CLUSTER == 0),
+            "%s: %d splits (takes 1 to %d, and multiples of %d up to %d)", who, n_splits, QD_CLUSTER, QD_CLUSTER, QD_CLUSTER * QD_MAX_GROUPS);
+  EL_REFUSE(n_splits <= QD_CLUSTER || part != nullptr, "%s: %d splits need the scratch", who, n_splits);
+  EL_REFUSE(n_splits <= QD_CLUSTER || nh <= 65535, "%s: too many heads", who);
   EL_REFUSE(window >= 0, "%s: a window of %d keys", who, window);
   EL_REFUSE((cos_t == nullptr) == (sin_t == nullptr) && (cos_t == nullptr || max_pos > 0), "%s: position tables", who);
   EL_REFUSE((uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0 && (uintptr_t)k_scale % 16 == 0 && (uintptr_t)v_scale % 16 == 0,
             "%s: the cache must start on 16-byte boundaries", who);
   EL_REFUSE((uintptr_t)out % 8 == 0 && ldo % 2 == 0, "%s: output rows must start on 8-byte boundaries", who);
-  const QuantDecodeArgs p = {q, out, (uint8_t*)kcache, (uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos_t, sin_t, err,
-                             ldq, ldo, table_stride, n_pages, max_pos, nh, nkv, window, meta_ready, scale};
-  // Four warps a block, three blocks an SM; eight warps where the blocks do not go round the SMs, so that as many copies are in flight.
-  const int warps = (long long)n_seqs * nkv * chunks * n_splits <= 148 ? 8 : 4;
+  const QuantDecodeArgs p = {q, out, (uint8_t*)kcache, (uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos_t, sin_t, err, part,
+                             ldq, ldo, table_stride, n_pages, max_pos, nh, nkv, window, meta_ready, n_splits < QD_CLUSTER ? n_splits : QD_CLUSTER, scale};
+  // Warps a block, by how many blocks there are: a block costs about 8 us from its first read to its last, whatever it has to do, so few
+  // blocks get many warps and many blocks few (an SM holds 12, 12 and 10 warps of them at a time).  us with 2, 4 and 12 warps: 2,048 blocks
+  // (64 sequences of 700 to 2,300 keys, 32 heads of 64) 87, 112, 132; 320 blocks (15 heads on 5) 34, 22, 26; 80 blocks (two splits of 8
+  // sequences of 130 to 2,040 keys, 15 heads on 5) 17, 11, 9.
+  const long long blocks = (long long)n_seqs * nkv * chunks * n_splits;
+  const int warps = blocks <= 148 ? QD_MAX_WARPS : blocks <= 592 ? 4 : 2;
   const int rc = format == QF_INT8 ? launch_decode_quant_int8(p, dtype, hd, n_seqs, n_splits, warps, stream)
                                    : launch_decode_quant_fp8(p, dtype, hd, n_seqs, n_splits, warps, stream);
   if (rc) return rc;

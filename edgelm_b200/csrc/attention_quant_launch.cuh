@@ -8,20 +8,19 @@
 
 namespace edgelm {
 
-// What a kernel needs once a device (a bit a device): shared memory, and clusters of more than 8 blocks.
+// What a kernel needs once a device (a bit a device): its shared memory.
 template <typename K>
-static cudaError_t quant_kernel_ready(K kern, int smem, bool wide_clusters, std::atomic<unsigned long long>& done) {
+static cudaError_t quant_kernel_ready(K kern, int smem, std::atomic<unsigned long long>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || (dev < 64 && done.load(std::memory_order_acquire) >> dev & 1)) return e;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   return e;
 }
 
 template <typename K, typename A>
-static cudaError_t launch_quant_kernel(K kern, dim3 grid, int threads, int smem, int pdl_bit, const A& p, cudaStream_t stream) {
+static cudaError_t launch_quant_kernel(K kern, dim3 grid, int cluster, int threads, int smem, int pdl_bit, const A& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -29,9 +28,9 @@ static cudaError_t launch_quant_kernel(K kern, dim3 grid, int threads, int smem,
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (grid.x > 1) {      // the blocks that share keys: a cluster
+  if (cluster > 1) {      // the blocks that share keys
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = grid.x;
+    attr[n].val.clusterDim.x = cluster;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
@@ -45,15 +44,20 @@ static cudaError_t launch_quant_kernel(K kern, dim3 grid, int threads, int smem,
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <int FMT, typename T, int HDT>
-static cudaError_t launch_decode_quant_one(const QuantDecodeArgs& p, int n_seqs, int n_splits, int warps, cudaStream_t stream) {
+template <int FMT, typename T, int HDT, int HC>
+static cudaError_t launch_decode_quant_heads(const QuantDecodeArgs& p, int n_seqs, int n_splits, int warps, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-  auto kern = attn_decode_quant_kernel<HDT, FMT, T>;
-  const cudaError_t e = quant_kernel_ready(kern, qd_smem(HDT, TERMS, QD_MAX_WARPS), true, done);
+  auto kern = attn_decode_quant_kernel<HDT, FMT, HC, T>;
+  const cudaError_t e = quant_kernel_ready(kern, qd_smem(HDT, TERMS, QD_MAX_WARPS), done);
   if (e != cudaSuccess) return e;
   const int chunks = (p.nh / p.nkv + QD_HEADS - 1) / QD_HEADS;
-  return launch_quant_kernel(kern, dim3(n_splits, p.nkv * chunks, n_seqs), warps * 32, qd_smem(HDT, TERMS, warps), 2, p, stream);
+  return launch_quant_kernel(kern, dim3(n_splits, p.nkv * chunks, n_seqs), p.cluster, warps * 32, qd_smem(HDT, TERMS, warps), 2, p, stream);
+}
+template <int FMT, typename T, int HDT>
+static cudaError_t launch_decode_quant_one(const QuantDecodeArgs& p, int n_seqs, int n_splits, int warps, cudaStream_t stream) {
+  return p.nh / p.nkv <= QD_HEADS / 2 ? launch_decode_quant_heads<FMT, T, HDT, 1>(p, n_seqs, n_splits, warps, stream)
+                                      : launch_decode_quant_heads<FMT, T, HDT, 2>(p, n_seqs, n_splits, warps, stream);
 }
 
 template <int FMT, typename T, int HDT>
@@ -61,9 +65,9 @@ static cudaError_t launch_prefill_quant_one(const QuantPrefillArgs& p, int n_til
   static std::atomic<unsigned long long> done{0};
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   auto kern = attn_prefill_quant_kernel<HDT, FMT, T>;
-  const cudaError_t e = quant_kernel_ready(kern, qp_smem(HDT, TERMS), false, done);
+  const cudaError_t e = quant_kernel_ready(kern, qp_smem(HDT, TERMS), done);
   if (e != cudaSuccess) return e;
-  return launch_quant_kernel(kern, dim3(n_splits, p.nkv, n_tiles * p.blocks_per_tile), QP_THREADS, qp_smem(HDT, TERMS), 16, p, stream);
+  return launch_quant_kernel(kern, dim3(n_splits, p.nkv, n_tiles * p.blocks_per_tile), n_splits, QP_THREADS, qp_smem(HDT, TERMS), 16, p, stream);
 }
 
 template <int FMT, typename T, int... I>
@@ -77,8 +81,15 @@ static cudaError_t launch_decode_quant_sizes(std::integer_sequence<int, I...>, c
 template <int FMT>
 static int launch_decode_quant(const QuantDecodeArgs& p, int dtype, int hd, int n_seqs, int n_splits, int warps, cudaStream_t stream) {
   const auto sizes = std::make_integer_sequence<int, 16>{};
-  const cudaError_t e = dtype == DT_F32 ? launch_decode_quant_sizes<FMT, float>(sizes, p, hd, n_seqs, n_splits, warps, stream)
-                                        : launch_decode_quant_sizes<FMT, __nv_bfloat16>(sizes, p, hd, n_seqs, n_splits, warps, stream);
+  cudaError_t e = dtype == DT_F32 ? launch_decode_quant_sizes<FMT, float>(sizes, p, hd, n_seqs, n_splits, warps, stream)
+                                  : launch_decode_quant_sizes<FMT, __nv_bfloat16>(sizes, p, hd, n_seqs, n_splits, warps, stream);
+  if (e == cudaSuccess && n_splits > p.cluster) {
+    const dim3 grid(n_seqs, p.nh), block((hd / 2 + 31) / 32 * 32);
+    const int groups = n_splits / p.cluster;
+    e = dtype == DT_F32 ? launch_pdl(2, attn_decode_quant_fold_kernel<float>, grid, block, (size_t)0, stream, (const float*)p.part, (float*)p.out, p.ldo, p.seq_pos, p.nh, hd, groups)
+                        : launch_pdl(2, attn_decode_quant_fold_kernel<__nv_bfloat16>, grid, block, (size_t)0, stream, (const float*)p.part, (__nv_bfloat16*)p.out, p.ldo, p.seq_pos,
+                                     p.nh, hd, groups);
+  }
   if (e != cudaSuccess) {
     set_error("attn_decode_quantized: launch failed: %s", cudaGetErrorString(e));
     return -2;

@@ -1549,14 +1549,14 @@ def softcap(z, cap):
 
 QUANT_FORMATS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 QUANT_PREFILL_TILE = 128   # new tokens per tile of the prompt attention over the 8-bit cache
-QUANT_MAX_SPLITS = 16      # blocks that share a sequence's keys in its decode attention (QD_MAX_SPLITS in attention_quant_decode.cuh)
+QUANT_CLUSTER = 8          # blocks of a cluster in the decode attention; 16 clusters at most share a sequence (attention_quant_decode.cuh)
 _QUANT_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
 # The library's functions of the 8-bit cache take one struct, laid out as in quant_cache.cu and attention_quant.cu (Q: pointers and pitches).
 _QUANT_APPEND = struct.Struct("@14Q9i").pack
 _QUANT_ROWS = struct.Struct("@12Q7i").pack
-_QUANT_DECODE = struct.Struct("@13Q2q12if").pack
+_QUANT_DECODE = struct.Struct("@14Q2q12if").pack
 _QUANT_PREFILL = struct.Struct("@14Q2q12if").pack
 
 
@@ -1669,18 +1669,25 @@ def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot,
 
 
 def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
-    """Blocks that share a sequence's keys in the decode attention over the 8-bit cache: enough for two an SM, as long as each of a
-    block's four warps can get a tile of keys (64, 32 or 16 by head size)."""
+    """Blocks that share a sequence's keys in the decode attention over the 8-bit cache: what one wave of blocks of eight warps, one an SM,
+    leaves free, as long as each warp can get a tile of keys (64, 32 or 16 by head size).  A quarter of the SMs stays out of the count:
+    clusters of 8 lie within a GPC, and 16 of them did not all find room at a time (16 heads on 4 of 128, 65,001 keys: 96 blocks 28 us,
+    128 blocks 43)."""
+    blocks = n_seqs * nkv * -(-(nh // nkv) // 8)
+    if blocks <= 0:
+        return 1
     tile = 64 if hd <= 64 else 32 if hd <= 128 else 16
-    blocks = max(1, n_seqs * nkv * -(-(nh // nkv) // 8))
-    splits = 1
-    while splits < QUANT_MAX_SPLITS and blocks * splits < 2 * n_sms and 4 * tile * splits < max_keys:
-        splits *= 2
-    return splits
+    splits = min(n_sms * 3 // 4 // blocks, max_keys // (8 * tile), 16 * QUANT_CLUSTER)
+    return max(1, splits if splits <= QUANT_CLUSTER else splits // QUANT_CLUSTER * QUANT_CLUSTER)
+
+
+def quantized_decode_scratch_floats(n_seqs, nh, hd, n_splits):
+    """Scratch of the decode attention over the 8-bit cache: clusters' partial results, if several share a sequence."""
+    return n_seqs * nh * (n_splits // QUANT_CLUSTER) * (hd + 2) if n_splits > QUANT_CLUSTER else 0
 
 
 def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv, hd, scale, n_splits,
-                           err, window, meta_ready):
+                           err, window, meta_ready, scratch):
     _heads(nh, nkv, hd, what)
     code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
     ldq, ldo, rows_q, rows_out = _quant_rows(q, out, nh * hd if cos is None else (nh + 2 * nkv) * hd, nh, hd, device, what)
@@ -1691,33 +1698,42 @@ def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_
     if n_splits is None:
         keys = page_table.shape[1] * PAGE
         n_splits = quantized_decode_splits(n_seqs, nh, nkv, hd, min(keys, window) if window > 0 else keys)
+    part = 0
+    if n_splits > QUANT_CLUSTER and n_seqs:
+        need = quantized_decode_scratch_floats(n_seqs, nh, hd, n_splits)
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+        if scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.get_device() != device:
+            raise KernelError(f"{what}: the scratch must be {need} contiguous float32 numbers on the cache's device")
+        part = scratch.data_ptr()
     cos_ptr = sin_ptr = max_pos = 0
     if cos is not None:
         max_pos = _quant_tables(cos, sin, hd, device, what)
         cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
     _call_packed("edgelm_attn_decode_quantized", _QUANT_DECODE(
         q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
-        seq_pos.data_ptr(), cos_ptr, sin_ptr, err.data_ptr() if err is not None else 0, _raw_stream(device), ldq, ldo, _dt(q), code, pitch, n_pages, max_pos,
-        n_seqs, nh, nkv, hd, n_splits, window, 1 if meta_ready else 0, scale), 1 if n_seqs else 0)
+        seq_pos.data_ptr(), cos_ptr, sin_ptr, err.data_ptr() if err is not None else 0, part, _raw_stream(device), ldq, ldo, _dt(q), code, pitch, n_pages, max_pos,
+        n_seqs, nh, nkv, hd, n_splits, window, 1 if meta_ready else 0, scale), (2 if part else 1) if n_seqs else 0)
 
 
 def attn_decode_quantized(q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, n_seqs, nh, nkv, hd, scale, n_splits=None,
-                          err=None, window=0, meta_ready=False):
+                          err=None, window=0, meta_ready=False, scratch=None):
     """`attn_decode` over the 8-bit cache: one new token per sequence, its query heads in q [n_seqs, nh * hd (or more)], its key and value
-    in the cache already.  `n_splits`: blocks that share a sequence's keys, 1 to 16 (None: by sizes, with the page table's width as
-    the longest sequence); their results meet on the chip, no scratch is taken.  A sequence with seq_pos < 0 has no token: its row
-    of `out` is zero.  `window`, `err`, `meta_ready`: as in `attn_decode`."""
+    in the cache already.  `n_splits`: blocks that share a sequence's keys, 1 to 8 or a multiple of 8 up to 128 (None: by sizes, with the
+    page table's width as the longest sequence).  Up to 8 their results meet on the chip; more need `scratch`, float32 room for
+    `quantized_decode_scratch_floats` (taken from torch when not given).  A sequence with seq_pos < 0 has no token: its row of `out`
+    is zero.  `window`, `err`, `meta_ready`: as in `attn_decode`."""
     _attn_decode_quantized("attn_decode_quantized", q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, None, None, n_seqs, nh, nkv, hd,
-                           scale, n_splits, err, window, meta_ready)
+                           scale, n_splits, err, window, meta_ready, scratch)
 
 
 def attn_decode_rope_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv, hd, scale,
-                               n_splits=None, err=None, window=0, meta_ready=False):
+                               n_splits=None, err=None, window=0, meta_ready=False, scratch=None):
     """`attn_decode_quantized` with the rotation and the append fused in: `qkv` holds the raw projections of one new token per sequence;
     the rotated keys and the values are written into the cache as codes, the same as `rope_quantize_append` writes."""
     _need(cos is not None and sin is not None, "attn_decode_rope_quantized: needs the position table")
     _attn_decode_quantized("attn_decode_rope_quantized", qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv,
-                           hd, scale, n_splits, err, window, meta_ready)
+                           hd, scale, n_splits, err, window, meta_ready, scratch)
 
 
 def quantized_prefill_splits(n_blocks, hd, max_keys, n_sms=148):

@@ -41,9 +41,13 @@ template <int FMT>
 __device__ __forceinline__ uint32_t to_codes4(float x0, float x1, float x2, float x3, float f) {
   if (f == 0.f) return 0u;
   const float y0 = __fmul_rn(x0, f), y1 = __fmul_rn(x1, f), y2 = __fmul_rn(x2, f), y3 = __fmul_rn(x3, f);
-  if (FMT == QF_INT8) {   // |y| <= 127 (1 + 2^-22): never past 127 once rounded
-    const int c0 = __float2int_rn(y0), c1 = __float2int_rn(y1), c2 = __float2int_rn(y2), c3 = __float2int_rn(y3);
-    return (uint32_t)(c0 & 255) | (uint32_t)(c1 & 255) << 8 | (uint32_t)(c2 & 255) << 16 | (uint32_t)(c3 & 255) << 24;
+  if (FMT == QF_INT8) {
+    // |y| <= 127 (1 + 2^-22): added to 1.5 2^23, whose last place is 1, it is rounded to a whole number, ties to even, and the low byte
+    // of the sum is that number (a conversion to int takes the special-function unit, a quarter as many a clock)
+    const float magic = 12582912.f;
+    const uint32_t c0 = __float_as_uint(__fadd_rn(y0, magic)), c1 = __float_as_uint(__fadd_rn(y1, magic));
+    const uint32_t c2 = __float_as_uint(__fadd_rn(y2, magic)), c3 = __float_as_uint(__fadd_rn(y3, magic));
+    return __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
   }
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y1), "f"(y0));

@@ -126,6 +126,8 @@ class Attention(Part):
         # 2 SMs + (sequences x kv heads), or three waves of resident blocks (`decode_splits`); up to 256 SMs
         cells = self.group * max(2 * 256 + n_seqs * self.nkv, 3 * 256 * (self._decode_resident() or 0))
         part = nbytes((cells * self.hd,), torch.float32) + nbytes((cells * 2,), torch.float32)
+        # (an 8-bit cache's: sequences x heads x clusters; its blocks, 8 a cluster, are at most one an SM, and one query head of a kv head's 8 has one)
+        part = max(part, nbytes((self.group * 256 // 8 * (self.hd + 2),), torch.float32))
         return qkv + out + h + part
 
     def _attend_decode(self, ctx, qkv, a, cache, table, tables):
@@ -155,10 +157,14 @@ class Attention(Part):
             linear.matmul(ctx, h, self.w_qkv, qkv, prefetch=(self.w_o,))
         if ctx.all_single:
             # one token per sequence: rotation, append and attention in one kernel
+            keys = table.shape[1] * ops.PAGE     # (fixed for a captured step, unlike the sequences' lengths)
+            splits = ops.quantized_decode_splits(ctx.n_seqs, self.nh, self.nkv, self.hd, min(keys, self.window or keys), ctx.n_sms)
+            room = ops.quantized_decode_scratch_floats(ctx.n_seqs, self.nh, self.hd, splits)
+            scratch = ctx.ws.alloc((room,), torch.float32) if room else None
             with ctx.prof("attn_decode"):
                 ops.attn_decode_rope_quantized(qkv, a, *kept, table, ctx.seq_index, ctx.seq_pos, *self.positions.rotation_tables(), ctx.n_seqs, self.nh,
-                                               self.nkv, self.hd, self.scale, err=ctx.err, window=self.window,
-                                               meta_ready=getattr(ctx, "metadata_precedes_kernels", False))
+                                               self.nkv, self.hd, self.scale, n_splits=splits, err=ctx.err, window=self.window,
+                                               meta_ready=getattr(ctx, "metadata_precedes_kernels", False), scratch=scratch)
             return
         with ctx.prof("rope_quantize_append"):
             self.positions.encode_and_quantize(ctx, qkv, cache, self.nh, self.nkv)

@@ -226,7 +226,7 @@ def test_decode_heads_and_lengths(fmt, dtype, nh, nkv, hd):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
-@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8, 16])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8, 16, 40, 128])
 @pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 1, 128), (11, 1, 256)])
 def test_decode_splits(fmt, splits, nh, nkv, hd):
     for fused in (False, True):
@@ -282,7 +282,7 @@ def test_decode_a_row_that_is_no_number_reaches_who_sees_it(fmt):
         cache["v"].view(torch.int8)[int(table[0, 1]), 0, 5] = 0
         cache["ks"][int(table[1, 0]), 1, 3] = float("nan")       # key of position 3, kv head 1
         cache["k"].view(torch.int8)[int(table[1, 0]), 1, 3] = 0
-    for splits in (1, 4):
+    for splits in (1, 4, 24):
         out, _, _ = decode_case(fmt, "bf16", 4, 2, 64, [130, 130, 130], change=change, spoil=False, splits=splits)
         nan = torch.isnan(out[:, :256].view(3, 4, 64)).all(-1)
         assert nan.tolist() == [[True, True, False, False], [False, False, True, True], [False] * 4]
@@ -310,6 +310,22 @@ def test_decode_rows_lie_where_the_strides_say():
     decode_case("int8", "bf16", 9, 3, 64, LENGTHS, q_pad=24)
     decode_case("fp8", "f32", 9, 3, 64, LENGTHS, q_pad=3, fused=True)
     decode_case("fp8", "bf16", 9, 3, 48, LENGTHS, q_pad=5, fused=True)
+
+
+def test_decode_scratch():
+    # one's own, of the size asked for; a smaller one is refused; results do not depend on what it held
+    cache, table = ref.make_cache("int8", 2, 64, [3000, 5, 0], DEV, 3)
+    q, outs = torch.randn((3, 4 * 64), device=DEV).bfloat16(), []
+    room = ops.quantized_decode_scratch_floats(3, 4, 64, 32)
+    assert room == 3 * 4 * 4 * 66 and ops.quantized_decode_scratch_floats(3, 4, 64, 8) == 0
+    for fill in (0.0, float("nan"), None):
+        scratch = torch.full((room,), fill, device=DEV) if fill is not None else None
+        outs.append(torch.empty((3, 256), dtype=torch.bfloat16, device=DEV))
+        ops.attn_decode_quantized(q, outs[-1], *cache_args(cache), table, i32(range(3)), i32([2999, 4, -1]), 3, 4, 2, 64, 0.125, n_splits=32, scratch=scratch)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and bool((outs[0][2] == 0).all())
+    with pytest.raises(ops.KernelError, match="scratch"):
+        ops.attn_decode_quantized(q, outs[0], *cache_args(cache), table, i32(range(3)), i32([2999, 4, -1]), 3, 4, 2, 64, 0.125, n_splits=32,
+                                  scratch=torch.empty(room - 1, device=DEV))
 
 
 def test_decode_repeats_itself_and_leaves_the_rest():

@@ -76,10 +76,10 @@ def test_the_library_refuses_too():
         return fn(packed)
 
     def go(dtype=0, fmt=0, n_seqs=1, nh=4, nkv=2, hd=64, splits=1, window=0, cos=0, sin=0, max_pos=0, k=256):
-        return run("edgelm_attn_decode_quantized", ops._QUANT_DECODE(256, 256, k, 256, 256, 256, 256, 256, 256, cos, sin, 0, 0, 512, 512, dtype, fmt, 1, 1, max_pos,
+        return run("edgelm_attn_decode_quantized", ops._QUANT_DECODE(256, 256, k, 256, 256, 256, 256, 256, 256, cos, sin, 0, 0, 0, 512, 512, dtype, fmt, 1, 1, max_pos,
                                                                      n_seqs, nh, nkv, hd, splits, window, 0, 0.1))
     assert go(n_seqs=0) == 0
-    for bad, word in (({"nh": 3}, "multiple"), ({"hd": 20}, "head size"), ({"fmt": 2}, "format"), ({"dtype": 5}, "dtype"), ({"splits": 17}, "splits"),
+    for bad, word in (({"nh": 3}, "multiple"), ({"hd": 20}, "head size"), ({"fmt": 2}, "format"), ({"dtype": 5}, "dtype"), ({"splits": 12}, "splits"), ({"splits": 136}, "splits"), ({"splits": 16}, "scratch"),
                       ({"splits": 0}, "splits"), ({"window": -1}, "window"), ({"cos": 256}, "tables"), ({"n_seqs": 70000}, "sequences"), ({"k": 264}, "16-byte")):
         assert go(**bad) < 0 and word in message(), (bad, message())
 
