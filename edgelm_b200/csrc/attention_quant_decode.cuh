@@ -264,7 +264,7 @@ attn_decode_quant_kernel(const QuantDecodeArgs p) {
         for (int i = 0; i < (HDT + 3) / 4; ++i) {
           const int j = lane + 32 * i;
           if (j < HALF) {
-            const uint32_t c = to_codes4<FMT>(a[i], b[i], 0.f, 0.f, rs.to_codes);
+            const uint32_t c = to_codes4<FMT>(make_float2(a[i], b[i]), make_float2(0.f, 0.f), rs.to_codes);
             fresh[(is_v ? HD : 0) + j] = (uint8_t)c;
             fresh[(is_v ? HD : 0) + j + HALF] = (uint8_t)(c >> 8);
             if (write) {

@@ -8,8 +8,8 @@
 //   quantized_rows         rows of given tokens as numbers, 16 codes a lane.
 //
 // Bound by memory where there are many tokens, and there by the chain position -> sequence -> slot -> page -> row that a lane walks
-// before it may write (or read) a row: a warp stays with one token, walks the chain once, and has up to four rows' pieces a lane on
-// their way at a time.  With few tokens a lane has one piece, so that the token is spread over more warps.
+// before it may write (or read) a row: a warp stays with one token, walks the chain once, and has two pieces a lane on their way
+// at a time.  With few tokens a lane has one piece, so that the token is spread over more warps.
 #include <type_traits>
 
 #include "quant_cache.cuh"
@@ -17,7 +17,7 @@
 namespace edgelm {
 
 constexpr int QA_THREADS = 256;
-constexpr int QA_MANY_PIECES = 4;
+constexpr int QA_MANY_PIECES = 2;
 constexpr int QA_MANY_TOKENS = 64;    // from here on QA_MANY_PIECES pieces a lane
 
 // Eight neighbouring numbers as they are stored.
@@ -25,13 +25,10 @@ template <typename T> struct Piece8;
 template <> struct Piece8<__nv_bfloat16> {
   uint4 v;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void get(float (&x)[8]) const {
+  __device__ __forceinline__ void get(float2 (&x)[4]) const {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i) x[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
 };
 template <> struct Piece8<float> {
@@ -40,23 +37,31 @@ template <> struct Piece8<float> {
     a = *reinterpret_cast<const float4*>(p);
     b = *reinterpret_cast<const float4*>(p + 4);
   }
-  __device__ __forceinline__ void get(float (&x)[8]) const {
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  __device__ __forceinline__ void get(float2 (&x)[4]) const {
+    x[0] = make_float2(a.x, a.y);
+    x[1] = make_float2(a.z, a.w);
+    x[2] = make_float2(b.x, b.y);
+    x[3] = make_float2(b.z, b.w);
   }
 };
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+__device__ __forceinline__ void store8(float* p, const float2 (&x)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float2 (&x)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[i].x, x[i].y);
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// the larger, or NaN if either is none
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 // The page of a token's position, or -1 (reported by one lane).
@@ -75,7 +80,7 @@ __device__ __forceinline__ int page_of_token(int pos, int max_pos, int seq, cons
 }
 
 template <typename T, int FMT, int LANES, int PIECES>   // LANES: lanes of a row (a power of two, at least hd / 16); PIECES a lane
-__global__ void __launch_bounds__(QA_THREADS)
+__global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 4 : 3)
 rope_quantize_append_kernel(T* __restrict__ qkv, T* __restrict__ q_out, const int32_t* __restrict__ tok_pos, const int32_t* __restrict__ tok_seq,
                             const int32_t* __restrict__ seq_slot, const int32_t* __restrict__ page_table, int table_stride, int n_pages,
                             const float* __restrict__ cos_t, const float* __restrict__ sin_t, int max_pos, uint8_t* __restrict__ kcache,
@@ -102,31 +107,41 @@ rope_quantize_append_kernel(T* __restrict__ qkv, T* __restrict__ q_out, const in
   const int pos = tok_pos[t];
   const int page = page_of_token(pos, max_pos, tok_seq[t], seq_slot, page_table, table_stride, n_pages, lane == 0 && chunk == 0, err);
   if (page < 0) return;                 // (whole warps: the token is the warp's)
-  float cs[8], sn[8];
+  float2 cs[4], sn[4];
   if (j < half) {
-    Piece8<float> c;
-    c.load(cos_t + (size_t)pos * half + j);
-    c.get(cs);
-    c.load(sin_t + (size_t)pos * half + j);
-    c.get(sn);
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      const float4 c = *reinterpret_cast<const float4*>(cos_t + (size_t)pos * half + j + 2 * k), s = *reinterpret_cast<const float4*>(sin_t + (size_t)pos * half + j + 2 * k);
+      cs[k] = make_float2(c.x, c.y);
+      cs[k + 1] = make_float2(c.z, c.w);
+      sn[k] = make_float2(s.x, s.y);
+      sn[k + 1] = make_float2(s.z, s.w);
+    }
   }
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int r = row0 + i * ROWS;
     const bool mine = r < rows && j < half;
-    float a[8] = {}, b[8] = {};
-    uint32_t most = 0;
+    float2 a[4] = {}, b[4] = {};
     if (mine) {
       lo[i].get(a);
       hi[i].get(b);
+      if (r < nh + nkv) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (r < nh + nkv) rotate_pair(a[k], b[k], cs[k], sn[k]);
-        most = max(most, max(magnitude_bits(a[k]), magnitude_bits(b[k])));
+        for (int k = 0; k < 4; ++k) {   // a c - b s, b c + a s, every product and sum rounded by itself
+          const float2 ac = mul2(a[k], cs[k]), bs = mul2(b[k], sn[k]), bc = mul2(b[k], cs[k]), as = mul2(a[k], sn[k]);
+          a[k] = make_float2(__fsub_rn(ac.x, bs.x), __fsub_rn(ac.y, bs.y));
+          b[k] = make_float2(__fadd_rn(bc.x, as.x), __fadd_rn(bc.y, as.y));
+        }
       }
     }
+    float most = 0.f;
+    if (row0 - lane / LANES + (i + 1) * ROWS > nh) {      // (the warp has rows that are kept)
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      for (int k = 0; k < 4; ++k) most = max_or_nan(max_or_nan(most, max_or_nan(fabsf(a[k].x), fabsf(a[k].y))), max_or_nan(fabsf(b[k].x), fabsf(b[k].y)));
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
     if (!mine) continue;
     if (r < nh) {
       T* dst = q_out ? q_out + ((size_t)t * nh + r) * hd + j : src + (size_t)r * hd;
@@ -134,19 +149,19 @@ rope_quantize_append_kernel(T* __restrict__ qkv, T* __restrict__ q_out, const in
       store8(dst + half, b);
       continue;
     }
-    const RowScale rs = row_scale<FMT>(most);
+    const RowScale rs = row_scale<FMT>(__float_as_uint(most));
     const bool is_v = r >= nh + nkv;
     const size_t at = ((size_t)page * nkv + (is_v ? r - nh - nkv : r - nh)) * PAGE + pos % PAGE;
     uint8_t* codes = (is_v ? vcache : kcache) + at * hd + j;
-    *reinterpret_cast<uint2*>(codes) = make_uint2(to_codes4<FMT>(a[0], a[1], a[2], a[3], rs.to_codes), to_codes4<FMT>(a[4], a[5], a[6], a[7], rs.to_codes));
-    *reinterpret_cast<uint2*>(codes + half) = make_uint2(to_codes4<FMT>(b[0], b[1], b[2], b[3], rs.to_codes), to_codes4<FMT>(b[4], b[5], b[6], b[7], rs.to_codes));
+    *reinterpret_cast<uint2*>(codes) = make_uint2(to_codes4<FMT>(a[0], a[1], rs.to_codes), to_codes4<FMT>(a[2], a[3], rs.to_codes));
+    *reinterpret_cast<uint2*>(codes + half) = make_uint2(to_codes4<FMT>(b[0], b[1], rs.to_codes), to_codes4<FMT>(b[2], b[3], rs.to_codes));
     if (part == 0) (is_v ? v_scale : k_scale)[at] = rs.scale;
   }
 }
 
 // keys[t], values[t] [nkv, hd] = the numbers that the cache holds for token t; a lane 16 of a row's at a time.
 template <typename T, int FMT, int PIECES>
-__global__ void __launch_bounds__(QA_THREADS)
+__global__ void __launch_bounds__(QA_THREADS, 6)
 quantized_rows_kernel(const uint8_t* __restrict__ kcache, const uint8_t* __restrict__ vcache, const float* __restrict__ k_scale,
                       const float* __restrict__ v_scale, const int32_t* __restrict__ tok_pos, const int32_t* __restrict__ tok_seq,
                       const int32_t* __restrict__ seq_slot, const int32_t* __restrict__ page_table, int table_stride, int n_pages,
@@ -183,17 +198,15 @@ quantized_rows_kernel(const uint8_t* __restrict__ kcache, const uint8_t* __restr
     const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float x[8] = {};
+      float2 x[4] = {};
       if (page >= 0) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           uint32_t p0, p1;
           codes_to_half<FMT>(w[2 * h + k], p0, p1);
-          const float2 f0 = half2_to_floats(p0), f1 = half2_to_floats(p1);
-          x[4 * k] = f0.x * scale[i];
-          x[4 * k + 1] = f0.y * scale[i];
-          x[4 * k + 2] = f1.x * scale[i];
-          x[4 * k + 3] = f1.y * scale[i];
+          const float2 s = make_float2(scale[i], scale[i]);
+          x[2 * k] = mul2(half2_to_floats(p0), s);
+          x[2 * k + 1] = mul2(half2_to_floats(p1), s);
         }
       }
       store8(dst + 8 * h, x);

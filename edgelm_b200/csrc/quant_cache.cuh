@@ -36,22 +36,31 @@ __device__ __forceinline__ RowScale row_scale(uint32_t largest_bits) {
   return {__fdiv_rn(a, quant_top<FMT>()), __fdiv_rn(quant_top<FMT>(), a)};
 }
 
+// Two products at a time, each rounded by itself.  (Sums that must not join such a product in one rounding are scalar: a packed product
+// followed by a packed sum was made one multiply-add here, explicit roundings notwithstanding.)
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // Four numbers of a row as four codes, the first in the lowest byte.
 template <int FMT>
-__device__ __forceinline__ uint32_t to_codes4(float x0, float x1, float x2, float x3, float f) {
+__device__ __forceinline__ uint32_t to_codes4(const float2& x0, const float2& x1, float f) {
   if (f == 0.f) return 0u;
-  const float y0 = __fmul_rn(x0, f), y1 = __fmul_rn(x1, f), y2 = __fmul_rn(x2, f), y3 = __fmul_rn(x3, f);
+  float2 y0 = mul2(x0, make_float2(f, f)), y1 = mul2(x1, make_float2(f, f));
   if (FMT == QF_INT8) {
     // |y| <= 127 (1 + 2^-22): added to 1.5 2^23, whose last place is 1, it is rounded to a whole number, ties to even, and the low byte
     // of the sum is that number (a conversion to int takes the special-function unit, a quarter as many a clock)
     const float magic = 12582912.f;
-    const uint32_t c0 = __float_as_uint(__fadd_rn(y0, magic)), c1 = __float_as_uint(__fadd_rn(y1, magic));
-    const uint32_t c2 = __float_as_uint(__fadd_rn(y2, magic)), c3 = __float_as_uint(__fadd_rn(y3, magic));
-    return __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
+    y0 = make_float2(__fadd_rn(y0.x, magic), __fadd_rn(y0.y, magic));
+    y1 = make_float2(__fadd_rn(y1.x, magic), __fadd_rn(y1.y, magic));
+    return __byte_perm(__byte_perm(__float_as_uint(y0.x), __float_as_uint(y0.y), 0x0040), __byte_perm(__float_as_uint(y1.x), __float_as_uint(y1.y), 0x0040), 0x5410);
   }
   uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y1), "f"(y0));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y3), "f"(y2));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y0.y), "f"(y0.x));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y1.y), "f"(y1.x));
   return (uint32_t)lo | (uint32_t)hi << 16;
 }
 
