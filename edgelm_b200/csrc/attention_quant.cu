@@ -1,4 +1,6 @@
 // Entry points of the attention over the 8-bit cache.
+#include <algorithm>
+
 #include "attention_quant_decode.cuh"
 #include "attention_quant_prefill.cuh"
 
@@ -11,7 +13,7 @@ bool prefill_quant_tc_takes(const void* q, long long ldq, const void* out, long 
 int launch_prefill_quant_tc(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache, const float* k_scale,
                             const float* v_scale, int format, const int32_t* page_table, int table_stride, int n_pages, const int32_t* seq_slot,
                             const int32_t* tile_seq, const int32_t* tile_tok0, const int32_t* tile_ntok, const int32_t* tile_pos0, int n_tiles,
-                            int max_tile_tokens, int nh, int nkv, int hd, float scale, int window, int* err, cudaStream_t stream);
+                            int max_tile_tokens, int nh, int nkv, int hd, float scale, int n_splits, int max_keys, int window, int* err, cudaStream_t stream);
 }  // namespace edgelm
 
 using namespace edgelm;
@@ -73,7 +75,8 @@ extern "C" int edgelm_attn_decode_quantized(const QuantDecodeCall* call) {
 }
 
 // New tokens, any number a sequence, as tiles of at most `max_tile_tokens` (up to 128) consecutive tokens of one sequence; their keys and
-// values are in the cache already.  n_splits: blocks that share a row tile's keys, 1 to 8 (mma.sync).  form: 0 by sizes, 1 mma.sync, 2 tcgen05.
+// values are in the cache already.  n_splits: blocks that share a row tile's keys, 1 to 8 (0: by sizes, with
+// `max_keys` as the longest sequence's keys that a token sees).  form: 0 tcgen05 where it takes the operands, else mma.sync; 1 mma.sync; 2 tcgen05.
 struct QuantPrefillCall {
   const void* q;
   void* out;
@@ -83,20 +86,21 @@ struct QuantPrefillCall {
   int* err;
   cudaStream_t stream;
   long long ldq, ldo;
-  int dtype, format, table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, n_splits, window, form;
+  int dtype, format, table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, n_splits, max_keys, window, form;
   float scale;
 };
 
 extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
   const auto [q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok, tile_pos0, err, stream, ldq, ldo, dtype, format,
-              table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, n_splits, window, form, scale] = *call;
+              table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, splits_wanted, max_keys, window, form, scale] = *call;
+  int n_splits = splits_wanted;
   if (n_tiles == 0) return 0;
   const char* who = "attn_prefill_quantized";
   EL_REFUSE(nh > 0 && nkv > 0 && nh % nkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, nh, nkv);
   EL_REFUSE(hd >= 16 && hd <= 256 && hd % 16 == 0, "%s: head size %d (takes 16..256 in steps of 16)", who, hd);
   EL_REFUSE((format == QF_INT8 || format == QF_FP8) && (dtype == DT_F32 || dtype == DT_BF16), "%s: format %d, dtype %d", who, format, dtype);
   EL_REFUSE(n_tiles > 0 && max_tile_tokens >= 1 && max_tile_tokens <= 128, "%s: %d tiles of up to %d tokens (takes 1 to 128)", who, n_tiles, max_tile_tokens);
-  EL_REFUSE(n_splits >= 1 && n_splits <= QP_MAX_SPLITS, "%s: %d splits (takes 1 to %d)", who, n_splits, QP_MAX_SPLITS);
+  EL_REFUSE(n_splits >= 0 && n_splits <= QP_MAX_SPLITS && max_keys >= 0, "%s: %d splits (takes 1 to %d, 0: by sizes), %d keys", who, n_splits, QP_MAX_SPLITS, max_keys);
   EL_REFUSE(window >= 0 && n_pages > 0, "%s: a window of %d keys, %d pages", who, window, n_pages);
   EL_REFUSE((uintptr_t)kcache % 16 == 0 && (uintptr_t)vcache % 16 == 0 && (uintptr_t)k_scale % 16 == 0 && (uintptr_t)v_scale % 16 == 0,
             "%s: the cache must start on 16-byte boundaries", who);
@@ -105,15 +109,19 @@ extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
   EL_REFUSE(form >= 0 && form <= 2, "%s: form %d", who, form);
   const bool tc = form != 1 && err != nullptr && prefill_quant_tc_takes(q, ldq, out, ldo, dtype, hd);
   EL_REFUSE(form != 2 || tc, "%s: these operands are not taken on tcgen05 (bfloat16, head size 64 or 128, 16-byte rows, an error word)", who);
-  if (form == 2 || (tc && max_tile_tokens * (nh / nkv) >= 128)) {
+  if (tc) {
     const int rc = launch_prefill_quant_tc(q, ldq, out, ldo, kcache, vcache, k_scale, v_scale, format, page_table, table_stride, n_pages, seq_slot, tile_seq,
-                                           tile_tok0, tile_ntok, tile_pos0, n_tiles, max_tile_tokens, nh, nkv, hd, scale, window, err, stream);
+                                           tile_tok0, tile_ntok, tile_pos0, n_tiles, max_tile_tokens, nh, nkv, hd, scale, n_splits, max_keys, window, err, stream);
     if (rc) return rc;
     EL_LAUNCH_CHECK(who);
     return 0;
   }
   const int per_tile = (max_tile_tokens * (nh / nkv) + QP_ROWS - 1) / QP_ROWS;
   EL_REFUSE(nkv <= 65535 && (long long)n_tiles * per_tile <= 65535, "%s: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", who, n_tiles, per_tile);
+  if (n_splits == 0) {      // (as on tcgen05: what a wave of blocks, one an SM at the least, leaves free, two tiles of keys each)
+    const long long blocks = (long long)nkv * n_tiles * per_tile;
+    n_splits = (int)std::max(1LL, std::min({(long long)QP_MAX_SPLITS, 148 / blocks, (long long)max_keys / (2 * (hd <= 128 ? 64 : 32))}));
+  }
   const QuantPrefillArgs p = {q, out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok,
                               tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, scale};
   const int rc = format == QF_INT8 ? launch_prefill_quant_int8(p, dtype, hd, n_tiles, n_splits, stream) : launch_prefill_quant_fp8(p, dtype, hd, n_tiles, n_splits, stream);

@@ -17,16 +17,21 @@
 // MN-major as they lie) and factors; warp 1 issues S = Q K^T, warp 2 O += P V with P out of tensor memory; warps 8 to 23 are the
 // softmax, four threads a row, a group each, which share the row's reference through shared memory.  S has two buffers of 128 columns,
 // so that S of block j + 1 is computed beside the softmax of block j; the weights go back over the scores that they came from.
+// Few rows over many keys (a short turn of a long conversation): a cluster of up to 8 blocks shares a row tile's key blocks, and the partial
+// results meet in distributed shared memory in a fixed order.
 // Every wait is bounded; where one runs out the block reports it, writes not-a-numbers and waits for what it has in flight before
 // it gives its memory back.
+#include <cooperative_groups.h>
 #include <math_constants.h>
+
+#include <algorithm>
 
 #include "attention_quant.cuh"
 #include "tc_common.cuh"
 
 namespace edgelm {
 
-constexpr int QT_ROWS = 128, QT_KEYS = 128, QT_THREADS = 768, QT_SOFT_WARPS = 16, QT_GROUPS = 4, QT_CONVERTERS = 4;
+constexpr int QT_ROWS = 128, QT_KEYS = 128, QT_THREADS = 768, QT_SOFT_WARPS = 16, QT_GROUPS = 4, QT_CONVERTERS = 4, QT_MAX_SPLITS = 8;
 constexpr int QT_TILE = 128 * 128;             // bytes of 128 rows of 64 float16
 constexpr float QT_LAZY = 8.f;
 constexpr int QT_SPREAD = 8;                   // powers of two between the scales of a group that tiles of scaled codes take
@@ -136,24 +141,33 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
   pdl_launch_dependents();      // (behind the allocation: a block of the next kernel must not hold tensor memory that this one waits for)
   pdl_wait();
 
-  const int g = a.nh / a.nkv, kvh = blockIdx.x, at = gridDim.y - 1 - blockIdx.y;      // (tiles of the most keys first)
+  const int splits = gridDim.x, split = blockIdx.x, g = a.nh / a.nkv, kvh = blockIdx.y, at = gridDim.z - 1 - blockIdx.z;      // (tiles of the most keys first)
   const int tile = at / a.blocks_per_tile, row_base = (at - tile * a.blocks_per_tile) * QT_ROWS;
   const int tok0 = a.tile_tok0[tile], rows_total = a.tile_ntok[tile] * g, pos0 = a.tile_pos0[tile];
   const int rows = min(QT_ROWS, rows_total - row_base);
   const int first_pos = pos0 + row_base / g, last_pos = pos0 + (row_base + max(rows, 1) - 1) / g;
   const int n_keys = last_pos + 1, page0 = a.window > 0 ? max(0, first_pos - a.window + 1) / PAGE : 0, n_pg = (n_keys + PAGE - 1) / PAGE - page0;
-  const int n_blk = rows > 0 ? (n_pg + 1) / 2 : 0;     // (no rows: a block of a tile that has fewer tokens than the longest)
-  auto key_of = [&](int j) { return (page0 + 2 * j) * PAGE; };
+  const int all_blk = rows > 0 ? (n_pg + 1) / 2 : 0;   // (no rows: a block of a tile that has fewer tokens than the longest)
+  const int n_blk = all_blk > split ? (all_blk - split + splits - 1) / splits : 0;     // this block's: split, split + splits, ..
+  auto pages_ahead = [&](int j) { return 2 * (split + j * splits); };                  // of the j-th of them, from page0 on
+  auto key_of = [&](int j) { return (page0 + pages_ahead(j)) * PAGE; };
   constexpr uint32_t S_COLS = 128, O_COL = 256;
   auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait_parked(smem_u32(bar), (uint32_t)parity, abort_flag, a.err)); };
 
+  // a block's results, where several share the rows: [128][dims, reference, sum], over its tiles of keys and values
+  constexpr int RESULT_PITCH = HD + 2;
+  static_assert(QT_ROWS * RESULT_PITCH * 4 <= (KS + VS) * KC * QT_TILE, "a block's results fit its tiles");
+  float* result = reinterpret_cast<float*>(k_s);
+
   if (n_blk == 0) {
+    if (splits > 1 && rows > 0)
+      for (int i = threadIdx.x; i < QT_ROWS * RESULT_PITCH; i += QT_THREADS) result[i] = i % RESULT_PITCH == HD ? -CUDART_INF_F : 0.f;
   } else if (warp == 0) {
     // ---- codes and scales: lanes 0 to 3 the block's first page, 4 to 7 its second
     const int32_t* pages = a.page_table + (size_t)a.seq_slot[a.tile_seq[tile]] * a.table_stride;
     auto page_of = [&](int j) {
-      const int i = page0 + 2 * j + (lane >> 2);
-      int page = lane < 8 && j < n_blk && 2 * j + (lane >> 2) < n_pg ? (i < a.table_stride ? pages[i] : -1) : 0;
+      const int ahead = pages_ahead(j) + (lane >> 2), i = page0 + ahead;
+      int page = lane < 8 && j < n_blk && ahead < n_pg ? (i < a.table_stride ? pages[i] : -1) : 0;
       if (page < 0 || page >= a.n_pages) {
         atomicOr(a.err, ERR_PAGE_RANGE);
         page = 0;                                  // (reported; some page is read in its place)
@@ -162,7 +176,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
     };
     int issued = 0, page = page_of(0);
     for (int j = 0; j < n_blk; ++j) {
-      const int st = j & 1, both = 2 * j + 1 < n_pg ? 2 : 1;
+      const int st = j & 1, both = pages_ahead(j) + 1 < n_pg ? 2 : 1;
       const int next = page_of(j + 1);
       if (j >= 2 && !wait(&c_empty[st], (j >> 1 & 1) ^ 1)) break;
       const uint32_t bar = smem_u32(&c_full[st]), dst = smem_u32(codes + st * Z::CODES);
@@ -477,9 +491,25 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
     if (ok) ok = wait(&o_done[(n_blk - 1) & 1], (n_blk - 1) >> 1 & 1);
     row_sum[part * QT_ROWS + row] = l;
     meet();
-    float inv = QT_OPERAND_BACK / ((row_sum[row] + row_sum[QT_ROWS + row]) + (row_sum[2 * QT_ROWS + row] + row_sum[3 * QT_ROWS + row]));
-    if (!ok) inv = CUDART_NAN_F;                   // a wait that ran out: nothing that could pass for a result
+    const float sum = ok ? (row_sum[row] + row_sum[QT_ROWS + row]) + (row_sum[2 * QT_ROWS + row] + row_sum[3 * QT_ROWS + row])
+                         : CUDART_NAN_F;           // a wait that ran out: nothing that could pass for a result
+    const float inv = QT_OPERAND_BACK / sum;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (splits > 1) {                              // (every MMA has read its tiles: the results take their place)
+      float* res = result + row * RESULT_PITCH;
+#pragma unroll
+      for (int c = 0; c < HD / 4; c += 8) {
+        uint32_t o[8];
+        tmem_ld8(tmem + lanes + O_COL + part * (HD / 4) + c, o);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 8; ++k) res[part * (HD / 4) + c + k] = __uint_as_float(o[k]);
+      }
+      if (part == 0) {
+        res[HD] = m;
+        res[HD + 1] = sum;
+      }
+    }
     __nv_bfloat16* dst = a.out + (size_t)(tok0 + tok) * a.ldo + (size_t)(kvh * g + rr - tok * g) * HD + part * (HD / 4);
 #pragma unroll
     for (int c = 0; c < HD / 4; c += 8) {
@@ -491,9 +521,44 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
         const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
         h[k] = *reinterpret_cast<const uint32_t*>(&y);
       }
-      if (mine) *reinterpret_cast<uint4*>(dst + c) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (mine && splits == 1) *reinterpret_cast<uint4*>(dst + c) = make_uint4(h[0], h[1], h[2], h[3]);
     }
     __syncwarp();
+  }
+  if (splits > 1 && rows > 0) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int it = split * QT_THREADS + threadIdx.x; it < rows * (HD / 2); it += splits * QT_THREADS) {
+      const int r = it / (HD / 2), d = (it - r * (HD / 2)) * 2;
+      float2 ml[QT_MAX_SPLITS], v[QT_MAX_SPLITS];
+#pragma unroll
+      for (int c = 0; c < QT_MAX_SPLITS; ++c) {
+        if (c < splits) {
+          const float* from = cluster.map_shared_rank(result, c) + r * RESULT_PITCH;
+          ml[c] = *reinterpret_cast<const float2*>(from + HD);
+          v[c] = *reinterpret_cast<const float2*>(from + d);
+        }
+      }
+      float M = -CUDART_INF_F, L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int c = 0; c < QT_MAX_SPLITS; ++c)
+        if (c < splits) M = fmaxf(M, ml[c].x);
+      const float ref = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll
+      for (int c = 0; c < QT_MAX_SPLITS; ++c) {
+        if (c < splits) {
+          const float f = aq_exp2(ml[c].x - ref);
+          L = fmaf(ml[c].y, f, L);
+          x = fmaf(v[c].x, f, x);
+          y = fmaf(v[c].y, f, y);
+        }
+      }
+      const float inv = QT_OPERAND_BACK / L;
+      const int row = row_base + r, t = row / g;
+      *reinterpret_cast<__nv_bfloat162*>(a.out + (size_t)(tok0 + t) * a.ldo + (size_t)(kvh * g + row - t * g) * HD + d) = __floats2bfloat162_rn(x * inv, y * inv);
+    }
+    cluster.sync();   // no block ends while another reads its result
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -504,13 +569,34 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
 }
 
 template <int HD, int FMT>
-static int launch_quant_tc(const QuantTcArgs& a, int n_tiles, cudaStream_t stream) {
+static int launch_quant_tc(const QuantTcArgs& a, int n_tiles, int n_splits, cudaStream_t stream) {
   constexpr int smem = QtSizes<HD>::smem;
   static_assert(smem <= 227 * 1024, "shared memory");
   auto kern = attn_prefill_quant_tc_kernel<HD, FMT>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   EL_REFUSE(e == cudaSuccess, "attn_prefill_quantized: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
-  launch_pdl(16, kern, dim3(a.nkv, n_tiles * a.blocks_per_tile), dim3(QT_THREADS), (size_t)smem, stream, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n_splits, a.nkv, n_tiles * a.blocks_per_tile);
+  cfg.blockDim = dim3(QT_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (n_splits > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = n_splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled() & 16) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t le = cudaLaunchKernelEx(&cfg, kern, a);
+  EL_REFUSE(le == cudaSuccess, "attn_prefill_quantized: launch failed: %s", cudaGetErrorString(le));
   return 0;
 }
 
@@ -522,13 +608,19 @@ bool prefill_quant_tc_takes(const void* q, long long ldq, const void* out, long 
 int launch_prefill_quant_tc(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache, const float* k_scale,
                             const float* v_scale, int format, const int32_t* page_table, int table_stride, int n_pages, const int32_t* seq_slot,
                             const int32_t* tile_seq, const int32_t* tile_tok0, const int32_t* tile_ntok, const int32_t* tile_pos0, int n_tiles,
-                            int max_tile_tokens, int nh, int nkv, int hd, float scale, int window, int* err, cudaStream_t stream) {
+                            int max_tile_tokens, int nh, int nkv, int hd, float scale, int n_splits, int max_keys, int window, int* err, cudaStream_t stream) {
   const int per_tile = (max_tile_tokens * (nh / nkv) + QT_ROWS - 1) / QT_ROWS;
   EL_REFUSE((long long)n_tiles * per_tile <= 65535, "attn_prefill_quantized: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", n_tiles, per_tile);
+  if (n_splits == 0) {
+    // Blocks that share a row tile's keys: what one wave of blocks, one an SM, leaves free (a quarter of the SMs stays out of the count: clusters
+    // lie within a GPC), as long as each has two blocks of keys.  17 new tokens of 9 heads of 64 on 3 behind 4,000: 1 split 54.7 us.
+    const long long blocks = (long long)nkv * n_tiles * per_tile;
+    n_splits = (int)std::max(1LL, std::min({(long long)QT_MAX_SPLITS, 111 / blocks, (long long)max_keys / (2 * QT_KEYS)}));
+  }
   const QuantTcArgs a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot,
                          tile_seq, tile_tok0, tile_ntok, tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, scale};
-  if (hd == 64) return format == QF_INT8 ? launch_quant_tc<64, QF_INT8>(a, n_tiles, stream) : launch_quant_tc<64, QF_FP8>(a, n_tiles, stream);
-  return format == QF_INT8 ? launch_quant_tc<128, QF_INT8>(a, n_tiles, stream) : launch_quant_tc<128, QF_FP8>(a, n_tiles, stream);
+  if (hd == 64) return format == QF_INT8 ? launch_quant_tc<64, QF_INT8>(a, n_tiles, n_splits, stream) : launch_quant_tc<64, QF_FP8>(a, n_tiles, n_splits, stream);
+  return format == QF_INT8 ? launch_quant_tc<128, QF_INT8>(a, n_tiles, n_splits, stream) : launch_quant_tc<128, QF_FP8>(a, n_tiles, n_splits, stream);
 }
 
 }  // namespace edgelm

@@ -1557,7 +1557,7 @@ _QUANT_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _QUANT_APPEND = struct.Struct("@14Q9i").pack
 _QUANT_ROWS = struct.Struct("@12Q7i").pack
 _QUANT_DECODE = struct.Struct("@14Q2q12if").pack
-_QUANT_PREFILL = struct.Struct("@14Q2q12if").pack
+_QUANT_PREFILL = struct.Struct("@14Q2q13if").pack
 
 
 def _call_packed(name, packed, launches):
@@ -1736,21 +1736,13 @@ def attn_decode_rope_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_
                            hd, scale, n_splits, err, window, meta_ready, scratch)
 
 
-def quantized_prefill_splits(n_blocks, hd, max_keys, n_sms=148):
-    """Blocks that share a row tile's keys in the prompt attention over the 8-bit cache, given how many there would be without."""
-    tile = 64 if hd <= 128 else 32
-    splits = 1
-    while splits < 8 and n_blocks * splits < n_sms and 2 * tile * splits < max_keys:
-        splits *= 2
-    return splits
-
-
 def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok, tile_pos0, n_tiles, nh, nkv,
                            hd, scale, err=None, window=0, max_keys=0, n_splits=None, form=0):
     """`attn_prefill` over the 8-bit cache: causal attention of new tokens (any number per sequence), as tiles of at most
     QUANT_PREFILL_TILE consecutive tokens of one sequence; the tokens' own keys and values are in the cache.  `max_keys`: the longest
     sequence's keys, if the caller knows them (0: the page table's width), by which the blocks that share keys are counted.
-    `form`: 0 by sizes, 1 on mma.sync, 2 on tcgen05 (bfloat16, head size 64 or 128, with the error word)."""
+    `form`: 0 on tcgen05 where it takes the operands (bfloat16, head size 64 or 128, 16-byte rows, with the error word), else on mma.sync;
+    1 on mma.sync; 2 on tcgen05.  `n_splits`: blocks that share a row tile's keys, 1 to 8 (None: by sizes)."""
     what = "attn_prefill_quantized"
     _heads(nh, nkv, hd, what)
     code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
@@ -1761,10 +1753,10 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     pitch = _quant_steps(page_table, wanted if err is None else wanted + ((err, 1),), device, what)
     window = int(window or 0)
     most = max(1, min(QUANT_PREFILL_TILE, rows_q))
-    if n_splits is None:
-        keys = max_keys or page_table.shape[1] * PAGE
-        n_splits = quantized_prefill_splits(nkv * n_tiles * -(-most * (nh // nkv) // 64), hd, min(keys, window + most) if window > 0 else keys)
+    keys = max_keys or page_table.shape[1] * PAGE
+    if window > 0:
+        keys = min(keys, window + most)
     _call_packed("edgelm_attn_prefill_quantized", _QUANT_PREFILL(
         qkv.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
         tile_seq.data_ptr(), tile_tok0.data_ptr(), tile_ntok.data_ptr(), tile_pos0.data_ptr(), err.data_ptr() if err is not None else 0, _raw_stream(device),
-        ldq, ldo, _dt(qkv), code, pitch, n_pages, n_tiles, most, nh, nkv, hd, n_splits, window, form, scale), 1 if n_tiles else 0)
+        ldq, ldo, _dt(qkv), code, pitch, n_pages, n_tiles, most, nh, nkv, hd, n_splits or 0, keys, window, form, scale), 1 if n_tiles else 0)

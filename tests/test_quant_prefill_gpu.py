@@ -82,7 +82,11 @@ def test_prompt_on_tcgen05(fmt, nh, nkv, hd):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 1, 128), (3, 1, 256)])
 def test_prompt_splits(splits, dtype, nh, nkv, hd):
-    prompt_case("int8", dtype, nh, nkv, hd, TOTALS + [2500], NEWS + [70], splits=splits)
+    prompt_case("int8", dtype, nh, nkv, hd, TOTALS + [2500], NEWS + [70], splits=splits, form=1)
+    if dtype == "bf16" and hd in (64, 128):
+        for window in (0, 300):
+            prompt_case("int8", dtype, nh, nkv, hd, TOTALS + [2500], NEWS + [70], splits=splits, form=2, window=window)
+            prompt_case("fp8", dtype, nh, nkv, hd, [2500, 40], [3, 40], splits=splits, form=2, window=window)
 
 
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 130, 5000])

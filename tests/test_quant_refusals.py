@@ -85,7 +85,7 @@ def test_the_library_refuses_too():
 
     def go2(dtype=0, fmt=0, n_tiles=1, most=128, nh=4, nkv=2, hd=64, splits=1, window=0, q=256, ldq=512, form=0):
         return run("edgelm_attn_prefill_quantized", ops._QUANT_PREFILL(q, 256, 256, 256, 256, 256, 256, 256, 256, 256, 256, 256, 0, 0, ldq, 512, dtype, fmt, 1, 1, n_tiles,
-                                                                       most, nh, nkv, hd, splits, window, form, 0.1))
+                                                                       most, nh, nkv, hd, splits, 64, window, form, 0.1))
     assert go2(n_tiles=0) == 0
     for bad, word in (({"nh": 3}, "multiple"), ({"hd": 20}, "head size"), ({"fmt": 2}, "format"), ({"most": 129}, "tokens"), ({"splits": 9}, "splits"),
                       ({"window": -1}, "window"), ({"form": 3}, "form"), ({"form": 2}, "tcgen05"), ({"q": 264}, "16-byte"), ({"ldq": 510}, "multiple of 4"),
