@@ -152,6 +152,8 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
   auto pages_ahead = [&](int j) { return 2 * (split + j * splits); };                  // of the j-th of them, from page0 on
   auto key_of = [&](int j) { return (page0 + pages_ahead(j)) * PAGE; };
   constexpr uint32_t S_COLS = 128, O_COL = 256;
+  // scores in units of log 2; the scale's sign (or a scale of 0) goes to the queries, so that the largest product has the largest weight
+  const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * AQ_LOG2E, turn = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
   auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, mbar_wait_parked(smem_u32(bar), (uint32_t)parity, abort_flag, a.err)); };
 
   // a block's results, where several share the rows: [128][dims, reference, sum], over its tiles of keys and values
@@ -265,12 +267,12 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       const float un_k = __uint_as_float((uint32_t)(254 - min(umax, 253)) << 23), un_e = __uint_as_float((uint32_t)(254 - min(vmax, 253)) << 23);
       float* kd = reinterpret_cast<float*>(key_data + (j & 3) * Z::KEY_DATA);
       if (lane == 0)
-        reinterpret_cast<float4*>(kd)[cw] = make_float4(1.0f / un_k * (a.scale * AQ_LOG2E), (float)(min(vmax, 253) - 127), un_e, slow ? 1.f : 0.f);
+        reinterpret_cast<float4*>(kd)[cw] = make_float4(1.0f / un_k * scale2, (float)(min(vmax, 253) - 127), un_e, slow ? 1.f : 0.f);
       float mk = fine ? u * un_k : CUDART_NAN_F, mv = fine ? v * un_e : 0.f;
       if (slow) {
         const ValueScale vsc = value_scale(fine ? v : 0.f);
         kd += QT_GROUPS * 4 + cw * 32 + lane;
-        kd[0] = fine ? u * (a.scale * AQ_LOG2E) : CUDART_NAN_F;
+        kd[0] = fine ? u * scale2 : CUDART_NAN_F;
         kd[QT_KEYS] = vsc.e;
         kd[2 * QT_KEYS] = vsc.f * (QT_OPERAND / AQ_OPERAND);
         kd[3 * QT_KEYS] = vsc.undo;
@@ -354,7 +356,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
         uint32_t h[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = aq_pack(__uint_as_float(w[k] << 16) * lift, __uint_as_float(w[k] & 0xffff0000u) * lift);
+        for (int k = 0; k < 4; ++k) h[k] = aq_pack(__uint_as_float(w[k] << 16) * (lift * turn), __uint_as_float(w[k] & 0xffff0000u) * (lift * turn));
         *reinterpret_cast<uint4*>(qt_place(q_s, row, part * (HD / 4) + 8 * i)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -370,28 +372,22 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       const float4* gd = reinterpret_cast<const float4*>(key_data + (j & 3) * Z::KEY_DATA);
       const ulonglong2* kd = reinterpret_cast<const ulonglong2*>(gd + QT_GROUPS) + part * 8;      // (slow) four keys' u; 32 further their e, f, 2^-e
       if (ok) ok = wait(&d_full[j & 3], j >> 2 & 1) && wait(&s_ready[b], j >> 1 & 1);
-      float x[32], mx = -CUDART_INF_F;
+      float x[32], f = 1.f, e = 0.f, mx = -CUDART_INF_F;
       float4 group = make_float4(0.f, 0.f, 0.f, 0.f);
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         group = gd[part];
         tmem_ld32(s_addr, reinterpret_cast<uint32_t*>(x));
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (group.w == 0.f) {
-          const float f = qf * group.x;
-          const uint64_t f2 = qt_pair(f, f), e2 = qt_pair(group.y, group.y);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 y = qt_unpair(qt_fma2(qt_pair(x[i], x[i + 1]), f2, e2));
-            x[i] = y.x;
-            x[i + 1] = y.y;
-          }
+        if (group.w == 0.f) {                      // x = f s + e, left to the exponent's multiply-add
+          f = fmaxf(qf * group.x, 1e-37f);         // (above zero: minus infinity times it stays so)
+          e = group.y;
         } else {
           const uint64_t f2 = qt_pair(qf, qf);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const ulonglong2 u = kd[i / 4], e = kd[32 + i / 4];
-            const float2 y = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i], x[i + 1]), u.x), f2, e.x)), z = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i + 2], x[i + 3]), u.y), f2, e.y));
+            const ulonglong2 u = kd[i / 4], o = kd[32 + i / 4];
+            const float2 y = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i], x[i + 1]), u.x), f2, o.x)), z = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i + 2], x[i + 3]), u.y), f2, o.y));
             x[i] = y.x;
             x[i + 1] = y.y;
             x[i + 2] = z.x;
@@ -412,7 +408,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
           mx = fmaxf(mx, fmaxf(x[i], x[i + 1]));
           mx1 = fmaxf(mx1, fmaxf(x[i + 2], x[i + 3]));
         }
-        mx = fmaxf(mx, mx1);
+        mx = fmaf(fmaxf(mx, mx1), f, e);
       }
       float* maxima = row_max + b * QT_GROUPS * QT_ROWS;
       maxima[part * QT_ROWS + row] = mx;
@@ -443,7 +439,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
         }
       }
       const float bias = AQ_LIFT - (m == -CUDART_INF_F ? 0.f : m);
-      const uint64_t bias2 = qt_pair(bias, bias);
+      const uint64_t f2 = qt_pair(f, f), bias2 = qt_pair(e + bias, e + bias);
       uint64_t sum0 = 0, sum1 = 0;
       if (group.w == 0.f) {
         const uint64_t operand2 = qt_pair(QT_OPERAND, QT_OPERAND);
@@ -452,7 +448,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
           uint32_t w[8];
 #pragma unroll
           for (int k = 0; k < 16; k += 2) {
-            const float2 y = qt_unpair(qt_add2(qt_pair(x[i + k], x[i + k + 1]), bias2));
+            const float2 y = qt_unpair(qt_fma2(qt_pair(x[i + k], x[i + k + 1]), f2, bias2));
             const uint64_t t = qt_pair(aq_exp2(y.x), aq_exp2(y.y));
             if (k & 2) sum1 = qt_add2(sum1, t);
             else sum0 = qt_add2(sum0, t);
@@ -470,7 +466,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
 #pragma unroll
           for (int k = 0; k < 16; k += 4) {
             const ulonglong2 f = kd[64 + (i + k) / 4], un = kd[96 + (i + k) / 4];
-            const float2 y = qt_unpair(qt_add2(qt_pair(x[i + k], x[i + k + 1]), bias2)), z = qt_unpair(qt_add2(qt_pair(x[i + k + 2], x[i + k + 3]), bias2));
+            const float2 y = qt_unpair(qt_fma2(qt_pair(x[i + k], x[i + k + 1]), f2, bias2)), z = qt_unpair(qt_fma2(qt_pair(x[i + k + 2], x[i + k + 3]), f2, bias2));
             const uint64_t t0 = qt_pair(aq_exp2(y.x), aq_exp2(y.y)), t1 = qt_pair(aq_exp2(z.x), aq_exp2(z.y));
             sum0 = qt_fma2(t0, un.x, sum0);
             sum1 = qt_fma2(t1, un.y, sum1);
@@ -613,9 +609,9 @@ int launch_prefill_quant_tc(const void* q, long long ldq, void* out, long long l
   EL_REFUSE((long long)n_tiles * per_tile <= 65535, "attn_prefill_quantized: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", n_tiles, per_tile);
   if (n_splits == 0) {
     // Blocks that share a row tile's keys: what one wave of blocks, one an SM, leaves free (a quarter of the SMs stays out of the count: clusters
-    // lie within a GPC), as long as each has two blocks of keys.  17 new tokens of 9 heads of 64 on 3 behind 4,000: 1 split 54.7 us.
+    // lie within a GPC), as long as each has a block of keys and more.  17 new tokens of 9 heads of 64 on 3 behind 4,000: 54.7 us with one block, 13.9 with 8.
     const long long blocks = (long long)nkv * n_tiles * per_tile;
-    n_splits = (int)std::max(1LL, std::min({(long long)QT_MAX_SPLITS, 111 / blocks, (long long)max_keys / (2 * QT_KEYS)}));
+    n_splits = (int)std::max(1LL, std::min({(long long)QT_MAX_SPLITS, 111 / blocks, (long long)max_keys / QT_KEYS - 1}));
   }
   const QuantTcArgs a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot,
                          tile_seq, tile_tok0, tile_ntok, tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, scale};

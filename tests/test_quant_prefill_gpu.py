@@ -166,3 +166,24 @@ def test_prompt_pages_that_are_not_there_are_reported():
         q = q.bfloat16()
         ops.attn_prefill_quantized(q, torch.empty_like(q), *cache_args(cache), table, i32([0]), *tiles, n, 2, 1, 64, 0.125, err=err, form=2)
         assert int(err) == 4
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_prompt_and_decode_scales_of_any_sign(scale):
+    nh, nkv, hd, n = 4, 2, 64, 150
+    cache, table = ref.make_cache("int8", nkv, hd, [n], DEV, 3)
+    q, err = torch.randn((n, nh * hd), generator=torch.Generator().manual_seed(4)).bfloat16().to(DEV), word()
+    keys, values = ref.sequence_rows(cache, table[0], n)
+    exact = ref.attend(q.double().view(n, nh, hd), 0, keys, values, scale)
+    bound = off_bound(q.double().view(n, nh, hd), 0, keys, values, abs(scale), 0, exact, torch.bfloat16, True)
+    # (the bound's weighted sum is the positive scale's; what any weights can do is at most the largest value)
+    bound = torch.maximum(bound, exact.abs() * 2.0 ** -8 + 2.0 ** -9 * values.abs().amax(0).repeat_interleave(nh // nkv, 0) * (1 + 40 * abs(scale)))
+    tiles, n_tiles = tiles_of([n], [n])
+    for form in (1, 2):
+        out = torch.empty_like(q)
+        ops.attn_prefill_quantized(q, out, *cache_args(cache), table, i32([0]), *tiles, n_tiles, nh, nkv, hd, scale, err=err, form=form)
+        check(out.view(n, nh, hd), exact, bound)
+    out = torch.empty((1, nh * hd), dtype=torch.bfloat16, device=DEV)
+    ops.attn_decode_quantized(q[n - 1:], out, *cache_args(cache), table, i32([0]), i32([n - 1]), 1, nh, nkv, hd, scale, err=err)
+    check(out.view(1, nh, hd), exact[n - 1:], bound[n - 1:])
+    assert int(err) == 0
