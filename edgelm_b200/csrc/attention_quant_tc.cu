@@ -43,7 +43,16 @@ template <int HD> struct QtSizes {
   static constexpr int CODES = QT_KEYS * (2 * HD + 8);        // a stage: key codes, value codes, key scales, value scales
   static constexpr int KEY_DATA = QT_GROUPS * 16 + 4 * QT_KEYS * 4;   // a block's groups {2^k scale log2(e), e, 2^-e, slow}, and of every key (where
                                                                       // its group is slow) u scale log2(e), e, f 2^-40, 2^-e; four blocks' worth
-  static constexpr int smem = 1024 + (KC + KS * KC + VS * KC) * QT_TILE + 2 * CODES + 4 * KEY_DATA + (2 + 1) * QT_GROUPS * QT_ROWS * 4 + 256;
+  // where things lie, from a 1,024-byte boundary on
+  static constexpr int KEYS = KC * QT_TILE, VALUES = KEYS + KS * KC * QT_TILE, CODES_AT = VALUES + VS * KC * QT_TILE, KEY_DATA_AT = CODES_AT + 2 * CODES;
+  static constexpr int ROW_MAX = KEY_DATA_AT + 4 * KEY_DATA;                      // [block & 1][group][128 rows]
+  static constexpr int ROW_SUM = ROW_MAX + 2 * QT_GROUPS * QT_ROWS * 4;           // [group][128 rows]
+  static constexpr int BARS = ROW_SUM + QT_GROUPS * QT_ROWS * 4;
+  static constexpr int N_BARS = 1 + 2 + 2 + 2 * KS + 2 * VS + 2 + 2 + 2 + 4 + 1;
+  static constexpr int smem = 1024 + BARS + N_BARS * 8 + 8;                       // (behind the barriers: the tensor memory's address and the abort flag)
+  static_assert(CODES % 16 == 0 && KEY_DATA % 16 == 0 && BARS % 8 == 0, "alignment");
+  // (two blocks of different clusters on one SM could each hold the tensor memory that the other's cluster waits for)
+  static_assert(2 * (smem + 1024) > 228 * 1024, "one block an SM");
 };
 
 // Instruction descriptor of kind::f16 with float16 operands: D float32, both K-major, M x N.
@@ -107,18 +116,18 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
   extern __shared__ uint8_t qt_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(qt_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* q_s = smem;                             // [KC][128 rows][128 bytes]
-  uint8_t* k_s = q_s + KC * QT_TILE;               // [KS][KC][128 keys][128 bytes]
-  uint8_t* v_s = k_s + KS * KC * QT_TILE;          // [VS][KC][128 keys][128 bytes]
-  uint8_t* codes = v_s + VS * KC * QT_TILE;        // [2][CODES]
-  uint8_t* key_data = codes + 2 * Z::CODES;        // [4][KEY_DATA]
-  float* row_max = reinterpret_cast<float*>(key_data + 4 * Z::KEY_DATA);      // [block & 1][group][128 rows]
-  float* row_sum = row_max + 2 * QT_GROUPS * QT_ROWS;      // [group][128 rows]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(row_sum + 2 * QT_ROWS);
+  uint8_t* k_s = smem + Z::KEYS;                   // [KS][KC][128 keys][128 bytes]
+  uint8_t* v_s = smem + Z::VALUES;                 // [VS][KC][128 keys][128 bytes]
+  uint8_t* codes = smem + Z::CODES_AT;             // [2][CODES]
+  uint8_t* key_data = smem + Z::KEY_DATA_AT;       // [4][KEY_DATA]
+  float* row_max = reinterpret_cast<float*>(smem + Z::ROW_MAX);
+  float* row_sum = reinterpret_cast<float*>(smem + Z::ROW_SUM);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Z::BARS);
   uint64_t *q_ready = bars, *c_full = bars + 1, *c_empty = c_full + 2, *k_full = c_empty + 2, *k_empty = k_full + KS, *v_full = k_empty + KS;
   uint64_t *v_empty = v_full + VS, *s_ready = v_empty + VS, *p_ready = s_ready + 2, *o_done = p_ready + 2;
   uint64_t* d_full = o_done + 2;                   // [4] key factors
   uint64_t* all_done = d_full + 4;                 // both issuers' MMAs
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Z::N_BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

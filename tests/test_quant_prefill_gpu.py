@@ -187,3 +187,19 @@ def test_prompt_and_decode_scales_of_any_sign(scale):
     ops.attn_decode_quantized(q[n - 1:], out, *cache_args(cache), table, i32([0]), i32([n - 1]), 1, nh, nkv, hd, scale, err=err)
     check(out.view(1, nh, hd), exact[n - 1:], bound[n - 1:])
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (16, 4, 128)])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_prompt_runs_over_and_over_agree(nh, nkv, hd, splits):
+    """Hundreds of launches in a row, blocks of one starting where blocks of the last end: every output the same, none reported."""
+    totals, news = [600, 130, 333, 520], [90, 65, 129, 31]
+    cache, table = ref.make_cache("int8", nkv, hd, totals, DEV, 3, k_size=1.5)
+    q = torch.randn((sum(news), nh * hd), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(DEV)
+    tiles, n_tiles = tiles_of(totals, news)
+    outs, err = torch.zeros((400,) + q.shape, dtype=q.dtype, device=DEV), word()
+    args = [*cache_args(cache), table, i32(range(4)), *tiles, n_tiles, nh, nkv, hd, 0.1]
+    for out in outs:
+        ops.attn_prefill_quantized(q, out, *args, err=err, n_splits=splits)
+    assert int(err) == 0 and bool(outs[0].isfinite().all())
+    assert bool((outs == outs[:1]).all())
