@@ -295,15 +295,19 @@ def test_decode_equal_scores_and_scores_far_apart():
     def far(cache, table):
         cache["ks"].mul_(200.0)
     decode_case("int8", "bf16", 4, 2, 64, [1, 130, 700], spoil=False, change=lambda c, t: c["ks"].zero_())
-    dtype = torch.float32
     cache, table = ref.make_cache("int8", 1, 64, [200], DEV, 5)
     cache["ks"].mul_(1e4)
-    q = torch.randn((1, 64), device=DEV)
-    out = torch.empty((1, 64), device=DEV)
-    ops.attn_decode_quantized(q, out, *cache_args(cache), table, i32([0]), i32([199]), 1, 1, 1, 64, 0.125)
     keys, values = ref.sequence_rows(cache, table[0], 200)
-    s = (keys[:, 0] @ q[0].double()) * 0.125
-    assert float(s.topk(2).values.diff().abs()) > 100 and torch.allclose(out[0].double(), values[int(s.argmax()), 0], rtol=2.0 ** -20, atol=0)
+    q = torch.randn((40, 64), generator=torch.Generator().manual_seed(6)).to(DEV)
+    apart = 0
+    for row in q.split(1):
+        out = torch.empty((1, 64), device=DEV)
+        ops.attn_decode_quantized(row, out, *cache_args(cache), table, i32([0]), i32([199]), 1, 1, 1, 64, 0.125)
+        s = (keys[:, 0] @ row[0].double()) * 0.125
+        if float(s.topk(2).values.diff().abs()) > 100:       # (the others' weights are below 2^-144 of the largest, none as operands)
+            apart += 1
+            assert torch.allclose(out[0].double(), values[int(s.argmax()), 0], rtol=2.0 ** -20, atol=0)
+    assert apart >= 20
 
 
 def test_decode_rows_lie_where_the_strides_say():
