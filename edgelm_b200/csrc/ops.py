@@ -1560,7 +1560,11 @@ _QUANT_DECODE = struct.Struct("@14Q2q12if").pack
 _QUANT_PREFILL = struct.Struct("@14Q2q13if").pack
 
 
-def _call_packed(name, packed, launches):
+def _call_packed(name, launches, pack, *args):
+    try:
+        packed = pack(*args)
+    except struct.error as e:      # a size beyond 32 bits, or no number at all
+        raise KernelError(f"{name[7:]}: {e}") from None
     fn = getattr(_lib or lib(), name)
     if fn.argtypes is None:
         fn.argtypes = [ctypes.c_char_p]
@@ -1632,7 +1636,8 @@ _raw_stream = torch._C._cuda_getCurrentRawStream     # a device's index -> the c
 
 def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, kcache, vcache, k_scale, v_scale, nh, nkv, hd, err, q_out=None):
     """`rope_kv_append` into the 8-bit cache: rotate q and k of the fused projection output in float32 (q back in place, or to `q_out`
-    [tokens, nh * hd] where given: `qkv` is then left as it was), write k and v as codes and scales into their pages."""
+    [tokens, nh * hd] where given: `qkv` is then left as it was), write k and v as codes and scales into their pages.  A position of a
+    sequence comes at most once a call (its row would be a mixture)."""
     what = "rope_quantize_append"
     _heads(nh, nkv, hd, what)
     code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
@@ -1644,10 +1649,10 @@ def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, 
         raise KernelError(f"{what}: q_out must be contiguous rows of {nh * hd} numbers, one per token, of the projections' type")
     max_pos = _quant_tables(cos, sin, hd, device, what)
     pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
-    _call_packed("edgelm_rope_quantize_append", _QUANT_APPEND(
+    _call_packed("edgelm_rope_quantize_append", 1 if T else 0, _QUANT_APPEND,
         qkv.data_ptr(), q_out.data_ptr() if q_out is not None else 0, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(),
         cos.data_ptr(), sin.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), err.data_ptr(), _raw_stream(device),
-        _dt(qkv), code, pitch, n_pages, max_pos, T, nh, nkv, hd), 1 if T else 0)
+        _dt(qkv), code, pitch, n_pages, max_pos, T, nh, nkv, hd)
 
 
 def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot, page_table, keys, values, err):
@@ -1663,9 +1668,9 @@ def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot,
     if not keys.get_device() == values.get_device() == device:
         raise KernelError(f"{what}: rows must lie on the cache's device")
     pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
-    _call_packed("edgelm_quantized_rows", _QUANT_ROWS(
+    _call_packed("edgelm_quantized_rows", 1 if T else 0, _QUANT_ROWS,
         kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(),
-        page_table.data_ptr(), keys.data_ptr(), values.data_ptr(), err.data_ptr(), _raw_stream(device), code, _dt(keys), pitch, n_pages, T, nkv, hd), 1 if T else 0)
+        page_table.data_ptr(), keys.data_ptr(), values.data_ptr(), err.data_ptr(), _raw_stream(device), code, _dt(keys), pitch, n_pages, T, nkv, hd)
 
 
 def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
@@ -1710,10 +1715,10 @@ def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_
     if cos is not None:
         max_pos = _quant_tables(cos, sin, hd, device, what)
         cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
-    _call_packed("edgelm_attn_decode_quantized", _QUANT_DECODE(
+    _call_packed("edgelm_attn_decode_quantized", (2 if part else 1) if n_seqs else 0, _QUANT_DECODE,
         q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
         seq_pos.data_ptr(), cos_ptr, sin_ptr, err.data_ptr() if err is not None else 0, part, _raw_stream(device), ldq, ldo, _dt(q), code, pitch, n_pages, max_pos,
-        n_seqs, nh, nkv, hd, n_splits, window, 1 if meta_ready else 0, scale), (2 if part else 1) if n_seqs else 0)
+        n_seqs, nh, nkv, hd, n_splits, window, 1 if meta_ready else 0, scale)
 
 
 def attn_decode_quantized(q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, n_seqs, nh, nkv, hd, scale, n_splits=None,
@@ -1756,7 +1761,7 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     keys = max_keys or page_table.shape[1] * PAGE
     if window > 0:
         keys = min(keys, window + most)
-    _call_packed("edgelm_attn_prefill_quantized", _QUANT_PREFILL(
+    _call_packed("edgelm_attn_prefill_quantized", 1 if n_tiles else 0, _QUANT_PREFILL,
         qkv.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
         tile_seq.data_ptr(), tile_tok0.data_ptr(), tile_ntok.data_ptr(), tile_pos0.data_ptr(), err.data_ptr() if err is not None else 0, _raw_stream(device),
-        ldq, ldo, _dt(qkv), code, pitch, n_pages, n_tiles, most, nh, nkv, hd, n_splits or 0, keys, window, form, scale), 1 if n_tiles else 0)
+        ldq, ldo, _dt(qkv), code, pitch, n_pages, n_tiles, most, nh, nkv, hd, n_splits or 0, keys, window, form, scale)

@@ -203,3 +203,30 @@ def test_prompt_runs_over_and_over_agree(nh, nkv, hd, splits):
         ops.attn_prefill_quantized(q, out, *args, err=err, n_splits=splits)
     assert int(err) == 0 and bool(outs[0].isfinite().all())
     assert bool((outs == outs[:1]).all())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,form", [("bf16", 2), ("bf16", 1), ("f32", 1)])
+def test_query_rows_that_are_no_numbers_stay_to_themselves(fmt, dtype, form):
+    """A head's query with a NaN or an infinity gives that head's row not-a-numbers, and changes no other row."""
+    nh, nkv, hd, totals, news = 4, 2, 64, [70, 200], [3, 40]
+    cache, table = ref.make_cache(fmt, nkv, hd, totals, DEV, 3)
+    clean = torch.randn((sum(news), nh, hd), generator=torch.Generator().manual_seed(4)).to(DTYPES[dtype]).to(DEV)
+    bad = clean.clone()
+    bad[1, 2, 5], bad[1, 0, 63], bad[20, 3, 0] = float("nan"), float("inf"), float("-inf")
+    hit = torch.zeros((sum(news), nh), dtype=torch.bool, device=DEV)
+    hit[1, 2] = hit[1, 0] = hit[20, 3] = True
+    tiles, n_tiles = tiles_of(totals, news)
+    outs = []
+    for q in (clean, bad):
+        out = torch.empty_like(q)
+        ops.attn_prefill_quantized(q.view(-1, nh * hd), out.view(-1, nh * hd), *cache_args(cache), table, i32(range(2)), *tiles, n_tiles, nh, nkv, hd, 0.1, err=word(),
+                                   form=form)
+        outs.append(out)
+    assert torch.equal(outs[1].isnan().all(-1), hit) and torch.equal(outs[0][~hit], outs[1][~hit]) and bool(outs[0].isfinite().all())
+    pos, outs = i32(n - 1 for n in totals), []
+    for q in (clean[:2], bad[:2]):
+        out = torch.empty_like(q)
+        ops.attn_decode_quantized(q.reshape(2, nh * hd), out.view(2, nh * hd), *cache_args(cache), table, i32(range(2)), pos, 2, nh, nkv, hd, 0.1)
+        outs.append(out)
+    assert torch.equal(outs[1].isnan().all(-1), hit[:2]) and torch.equal(outs[0][~hit[:2]], outs[1][~hit[:2]]) and bool(outs[0].isfinite().all())

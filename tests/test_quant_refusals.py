@@ -103,3 +103,11 @@ def test_the_library_refuses_too():
     assert go4(n=0) == 0
     for bad, word in (({"nkv": 0}, "sizes"), ({"hd": 40}, "head size"), ({"fmt": 3}, "format"), ({"dtype": 2}, "dtype"), ({"keys": 260}, "16-byte"), ({"n": 1 << 30}, "grid")):
         assert go4(**bad) < 0 and word in message(), (bad, message())
+
+
+def test_numbers_that_no_field_holds():
+    for field, value in ((18, 1 << 31), (18, 64.5), (0, -1)):
+        args = [0] * 19
+        args[field] = value
+        with pytest.raises(ops.KernelError, match="quantized_rows"):
+            ops._call_packed("edgelm_quantized_rows", 0, ops._QUANT_ROWS, *args)
