@@ -92,8 +92,7 @@ struct QuantPrefillCall {
 
 extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
   const auto [q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok, tile_pos0, err, stream, ldq, ldo, dtype, format,
-              table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, splits_wanted, max_keys, window, form, scale] = *call;
-  int n_splits = splits_wanted;
+              table_stride, n_pages, n_tiles, max_tile_tokens, nh, nkv, hd, n_splits, max_keys, window, form, scale] = *call;
   if (n_tiles == 0) return 0;
   const char* who = "attn_prefill_quantized";
   EL_REFUSE(nh > 0 && nkv > 0 && nh % nkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, nh, nkv);
@@ -118,12 +117,8 @@ extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
   }
   const int per_tile = (max_tile_tokens * (nh / nkv) + QP_ROWS - 1) / QP_ROWS;
   EL_REFUSE(nkv <= 65535 && (long long)n_tiles * per_tile <= 65535, "%s: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", who, n_tiles, per_tile);
-  if (n_splits == 0) {      // (as on tcgen05: what a wave of blocks, one an SM at the least, leaves free, two tiles of keys each)
-    const long long blocks = (long long)nkv * n_tiles * per_tile;
-    n_splits = (int)std::max(1LL, std::min({(long long)QP_MAX_SPLITS, 148 / blocks, (long long)max_keys / (2 * (hd <= 128 ? 64 : 32))}));
-  }
   const QuantPrefillArgs p = {q, out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok,
-                              tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, scale};
+                              tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, max_keys, scale};
   const int rc = format == QF_INT8 ? launch_prefill_quant_int8(p, dtype, hd, n_tiles, n_splits, stream) : launch_prefill_quant_fp8(p, dtype, hd, n_tiles, n_splits, stream);
   if (rc) return rc;
   EL_LAUNCH_CHECK(who);

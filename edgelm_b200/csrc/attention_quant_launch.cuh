@@ -1,5 +1,6 @@
 // Host side of the attention over the 8-bit cache: one instantiation a head size, format and type (a source file a kernel and format).
 #pragma once
+#include <algorithm>
 #include <atomic>
 #include <utility>
 
@@ -65,8 +66,23 @@ static cudaError_t launch_prefill_quant_one(const QuantPrefillArgs& p, int n_til
   static std::atomic<unsigned long long> done{0};
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   auto kern = attn_prefill_quant_kernel<HDT, FMT, T>;
-  const cudaError_t e = quant_kernel_ready(kern, qp_smem(HDT, TERMS), done);
+  cudaError_t e = quant_kernel_ready(kern, qp_smem(HDT, TERMS), done);
   if (e != cudaSuccess) return e;
+  if (n_splits == 0) {
+    // Blocks that share a row tile's keys: as many as make one wave, two tiles of keys each at the least; or up to two waves where each
+    // has four (the last rows of a prompt see twice the average's keys, and the tiles of the most keys go first).  us with 1, 2, 3 and 8 blocks,
+    // float32: 180 row tiles of up to 701 keys (9 heads of 64 on 3) 30, 22, 23, 52; 288 of up to 2,000 85, 55, 69, 121; 432 of up to
+    // 300 23, 33, 40, 107; 96 of 1,600 to 1,700 (16 heads of 128 on 4) 93, 93, 72, 114.
+    static std::atomic<int> resident{0};
+    int per_sm = resident.load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+      if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, QP_THREADS, qp_smem(HDT, TERMS))) != cudaSuccess) return e;
+      resident.store(per_sm, std::memory_order_relaxed);
+    }
+    const long long blocks = (long long)p.nkv * n_tiles * p.blocks_per_tile, wave = 148LL * per_sm, tiles = p.max_keys / qp_tile_keys(HDT);
+    const long long one = std::min(wave / blocks, tiles / 2), two = std::min((2 * wave + blocks / 2) / blocks, tiles / 4);
+    n_splits = (int)std::max(1LL, std::min((long long)QP_MAX_SPLITS, std::max(one, two)));
+  }
   return launch_quant_kernel(kern, dim3(n_splits, p.nkv, n_tiles * p.blocks_per_tile), n_splits, QP_THREADS, qp_smem(HDT, TERMS), 16, p, stream);
 }
 
