@@ -107,7 +107,7 @@ extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
   EL_REFUSE((uintptr_t)out % 8 == 0 && ldo % 2 == 0, "%s: output rows must start on 8-byte boundaries", who);
   EL_REFUSE(form >= 0 && form <= 2, "%s: form %d", who, form);
   const bool tc = form != 1 && err != nullptr && prefill_quant_tc_takes(q, ldq, out, ldo, dtype, hd);
-  EL_REFUSE(form != 2 || tc, "%s: these operands are not taken on tcgen05 (bfloat16, head size 64 or 128, 16-byte rows, an error word)", who);
+  EL_REFUSE(form != 2 || tc, "%s: these operands are not taken on tcgen05 (bfloat16, head size up to 128, 16-byte rows, an error word)", who);
   if (tc) {
     const int rc = launch_prefill_quant_tc(q, ldq, out, ldo, kcache, vcache, k_scale, v_scale, format, page_table, table_stride, n_pages, seq_slot, tile_seq,
                                            tile_tok0, tile_ntok, tile_pos0, n_tiles, max_tile_tokens, nh, nkv, hd, scale, n_splits, max_keys, window, err, stream);

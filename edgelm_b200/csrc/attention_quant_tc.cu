@@ -1,5 +1,5 @@
 // Causal attention of many new tokens over the 8-bit cache on the fifth-generation tensor cores (tcgen05): bfloat16 models, head
-// sizes 64 and 128.  The other head sizes, float32 models and short steps stay on mma.sync (attention_quant_prefill.cuh).
+// sizes up to 128.  The other head sizes, float32 models and short steps stay on mma.sync (attention_quant_prefill.cuh).
 //
 // The tensor cores take float16 operands, so the codes become float16 on the chip.  Scales are applied 32 keys (a group) at a time: with
 // 2^k and 2^e the largest powers of two in the group's key and value scales, the tiles hold a_j (u_j / 2^k) and c_j (v_j / 2^e), one more
@@ -25,6 +25,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "attention_quant.cuh"
 #include "tc_common.cuh"
@@ -38,7 +39,7 @@ constexpr int QT_SPREAD = 8;                   // powers of two between the scal
 constexpr float QT_OPERAND = 9.094947017729282e-13f, QT_OPERAND_BACK = 1099511627776.f;    // 2^-40, 2^40
 
 template <int HD> struct QtSizes {
-  static constexpr int KC = HD / 64;                          // tiles of 64 dims
+  static constexpr int KC = (HD + 63) / 64;                   // tiles of 64 dims (what lies behind a row's end in the last is not read, or its products are not)
   static constexpr int KS = 2, VS = KC == 1 ? 2 : 1;          // stages of keys and values (shared memory has room for one of values at 128)
   static constexpr int CODES = QT_KEYS * (2 * HD + 8);        // a stage: key codes, value codes, key scales, value scales
   static constexpr int KEY_DATA = QT_GROUPS * 16 + 4 * QT_KEYS * 4;   // a block's groups {2^k scale log2(e), e, 2^-e, slow}, and of every key (where
@@ -49,9 +50,10 @@ template <int HD> struct QtSizes {
   static constexpr int ROW_SUM = ROW_MAX + 2 * QT_GROUPS * QT_ROWS * 4;           // [group][128 rows]
   static constexpr int BARS = ROW_SUM + QT_GROUPS * QT_ROWS * 4;
   static constexpr int N_BARS = 1 + 2 + 2 + 2 * KS + 2 * VS + 2 + 2 + 2 + 4 + 1;
-  static constexpr int smem = 1024 + BARS + N_BARS * 8 + 8;                       // (behind the barriers: the tensor memory's address and the abort flag)
+  static constexpr int needed = 1024 + BARS + N_BARS * 8 + 8;                     // (behind the barriers: the tensor memory's address and the abort flag)
+  // one block an SM: two blocks of different clusters on one SM could each hold the tensor memory that the other's cluster waits for
+  static constexpr int smem = needed > 114 * 1024 ? needed : 114 * 1024;
   static_assert(CODES % 16 == 0 && KEY_DATA % 16 == 0 && BARS % 8 == 0, "alignment");
-  // (two blocks of different clusters on one SM could each hold the tensor memory that the other's cluster waits for)
   static_assert(2 * (smem + 1024) > 228 * 1024, "one block an SM");
 };
 
@@ -256,8 +258,8 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
     qt_drain(smem_u32(all_done), 0);
   } else if (warp >= 4 && warp < 8) {
     // ---- 32 keys a warp: their factors, and their codes as float16 tiles
-    constexpr int PER_ROW = HD / 16, ROWS = 32 / PER_ROW;             // pieces of 16 codes; rows of a pass
-    const int cw = warp - 4, sub = lane / PER_ROW, d = lane % PER_ROW * 16;
+    constexpr int PER_ROW = HD / 16;                                  // pieces of 16 codes, and passes over the warp's rows
+    const int cw = warp - 4;
     for (int j = 0; j < n_blk; ++j) {
       const int cs = j & 1, ks = j % KS, vs = j % VS;
       if (!wait(&c_full[cs], j >> 1 & 1)) break;
@@ -290,16 +292,16 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       const __half2 hk = __float2half2_rn(mk), hv = __float2half2_rn(mv);
       const uint32_t fk = *reinterpret_cast<const uint32_t*>(&hk), fv = *reinterpret_cast<const uint32_t*>(&hv);
       auto tile = [&](const uint8_t* from, uint8_t* to, uint32_t factor, bool values) {
-        uint4 c[32 / ROWS];
+        uint4 c[PER_ROW];
 #pragma unroll
-        for (int i = 0; i < 32 / ROWS; ++i) {
-          const int r = i * ROWS + sub;
+        for (int i = 0; i < PER_ROW; ++i) {
+          const int r = (i * 32 + lane) / PER_ROW, d = (i * 32 + lane) % PER_ROW * 16;
           c[i] = *reinterpret_cast<const uint4*>(from + r * HD + d);
           if (values && key_of(j) + cw * 32 + r >= n_keys) c[i] = make_uint4(0, 0, 0, 0);      // whatever lies there, it meets weights of zero as zero
         }
 #pragma unroll
-        for (int i = 0; i < 32 / ROWS; ++i) {
-          const int r = i * ROWS + sub;
+        for (int i = 0; i < PER_ROW; ++i) {
+          const int r = (i * 32 + lane) / PER_ROW, d = (i * 32 + lane) % PER_ROW * 16;
           const uint32_t fr = __shfl_sync(0xffffffffu, factor, r);
           uint32_t w[8];
           codes_to_half<FMT>(c[i].x, w[0], w[1]);
@@ -338,16 +340,16 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
     const bool mine = row < rows;
     auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(quarter + 1) : "memory"); };      // the row's four threads (warps w, w + 4, w + 8, w + 12)
     auto all_four = [&](const float* at) { return fmaxf(fmaxf(at[row], at[QT_ROWS + row]), fmaxf(at[2 * QT_ROWS + row], at[3 * QT_ROWS + row])); };
-    // ---- this thread's quarter of its query row as float16 numbers, lifted by a power of two (exact)
+    // ---- this thread's pieces of eight numbers of its row (part, part + 4, ..) as float16 numbers, lifted by a power of two (exact)
+    constexpr int PIECES = HD / 8, N = (PIECES + 3) / 4;
     float qf;
     {
-      constexpr int N = HD / 32;                   // pieces of eight numbers
       uint4 v[N];
       uint32_t most = 0;
-      const __nv_bfloat16* src = a.q + (size_t)(tok0 + tok) * a.ldq + (size_t)(kvh * g + rr - tok * g) * HD + part * (HD / 4);
+      const __nv_bfloat16* src = a.q + (size_t)(tok0 + tok) * a.ldq + (size_t)(kvh * g + rr - tok * g) * HD;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        v[i] = mine ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
+        v[i] = mine && part + 4 * i < PIECES ? *reinterpret_cast<const uint4*>(src + 8 * (part + 4 * i)) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) most = max(most, max(w[k] << 16 & 0x7fffffffu, w[k] & 0x7fff0000u));
@@ -366,7 +368,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
         uint32_t h[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) h[k] = aq_pack(__uint_as_float(w[k] << 16) * (lift * turn), __uint_as_float(w[k] & 0xffff0000u) * (lift * turn));
-        *reinterpret_cast<uint4*>(qt_place(q_s, row, part * (HD / 4) + 8 * i)) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (part + 4 * i < PIECES) *reinterpret_cast<uint4*>(qt_place(q_s, row, 8 * (part + 4 * i))) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -437,9 +439,9 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
         if (!ok) continue;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < HD / 4; c += 8) {
+        for (int c = part; c < PIECES; c += 4) {
           uint32_t o[8];
-          const uint32_t o_addr = tmem + lanes + O_COL + part * (HD / 4) + c;
+          const uint32_t o_addr = tmem + lanes + O_COL + 8 * c;
           tmem_ld8(o_addr, o);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
@@ -503,30 +505,30 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
     if (splits > 1) {                              // (every MMA has read its tiles: the results take their place)
       float* res = result + row * RESULT_PITCH;
 #pragma unroll
-      for (int c = 0; c < HD / 4; c += 8) {
+      for (int c = part; c < PIECES; c += 4) {
         uint32_t o[8];
-        tmem_ld8(tmem + lanes + O_COL + part * (HD / 4) + c, o);
+        tmem_ld8(tmem + lanes + O_COL + 8 * c, o);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int k = 0; k < 8; ++k) res[part * (HD / 4) + c + k] = __uint_as_float(o[k]);
+        for (int k = 0; k < 8; ++k) res[8 * c + k] = __uint_as_float(o[k]);
       }
       if (part == 0) {
         res[HD] = m;
         res[HD + 1] = sum;
       }
     }
-    __nv_bfloat16* dst = a.out + (size_t)(tok0 + tok) * a.ldo + (size_t)(kvh * g + rr - tok * g) * HD + part * (HD / 4);
+    __nv_bfloat16* dst = a.out + (size_t)(tok0 + tok) * a.ldo + (size_t)(kvh * g + rr - tok * g) * HD;
 #pragma unroll
-    for (int c = 0; c < HD / 4; c += 8) {
+    for (int c = part; c < PIECES; c += 4) {
       uint32_t o[8], h[4];
-      tmem_ld8(tmem + lanes + O_COL + part * (HD / 4) + c, o);
+      tmem_ld8(tmem + lanes + O_COL + 8 * c, o);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
         h[k] = *reinterpret_cast<const uint32_t*>(&y);
       }
-      if (mine && splits == 1) *reinterpret_cast<uint4*>(dst + c) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (mine && splits == 1) *reinterpret_cast<uint4*>(dst + 8 * c) = make_uint4(h[0], h[1], h[2], h[3]);
     }
     __syncwarp();
   }
@@ -605,9 +607,17 @@ static int launch_quant_tc(const QuantTcArgs& a, int n_tiles, int n_splits, cuda
   return 0;
 }
 
+template <int... I>
+static int launch_quant_tc_sizes(std::integer_sequence<int, I...>, const QuantTcArgs& a, int format, int hd, int n_tiles, int n_splits, cudaStream_t stream) {
+  int rc = -1;
+  ((hd == 16 * (I + 1) ? (void)(rc = format == QF_INT8 ? launch_quant_tc<16 * (I + 1), QF_INT8>(a, n_tiles, n_splits, stream)
+                                                       : launch_quant_tc<16 * (I + 1), QF_FP8>(a, n_tiles, n_splits, stream)) : (void)0), ...);
+  return rc;
+}
+
 // Rows of the operands are checked by the entry point (attention_quant.cu); this form also wants 16-byte rows of queries and outputs.
 bool prefill_quant_tc_takes(const void* q, long long ldq, const void* out, long long ldo, int dtype, int hd) {
-  return dtype == DT_BF16 && (hd == 64 || hd == 128) && (uintptr_t)q % 16 == 0 && ldq % 8 == 0 && (uintptr_t)out % 16 == 0 && ldo % 8 == 0;
+  return dtype == DT_BF16 && hd % 16 == 0 && hd >= 16 && hd <= 128 && (uintptr_t)q % 16 == 0 && ldq % 8 == 0 && (uintptr_t)out % 16 == 0 && ldo % 8 == 0;
 }
 
 int launch_prefill_quant_tc(const void* q, long long ldq, void* out, long long ldo, const void* kcache, const void* vcache, const float* k_scale,
@@ -624,8 +634,7 @@ int launch_prefill_quant_tc(const void* q, long long ldq, void* out, long long l
   }
   const QuantTcArgs a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot,
                          tile_seq, tile_tok0, tile_ntok, tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, scale};
-  if (hd == 64) return format == QF_INT8 ? launch_quant_tc<64, QF_INT8>(a, n_tiles, n_splits, stream) : launch_quant_tc<64, QF_FP8>(a, n_tiles, n_splits, stream);
-  return format == QF_INT8 ? launch_quant_tc<128, QF_INT8>(a, n_tiles, n_splits, stream) : launch_quant_tc<128, QF_FP8>(a, n_tiles, n_splits, stream);
+  return launch_quant_tc_sizes(std::make_integer_sequence<int, 8>{}, a, format, hd, n_tiles, n_splits, stream);
 }
 
 }  // namespace edgelm

@@ -67,7 +67,7 @@ def test_prompt_heads_and_lengths(fmt, dtype, nh, nkv, hd):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
-@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 4, 64), (12, 1, 64), (4, 1, 128), (3, 3, 128), (32, 2, 128)])
+@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 4, 64), (12, 1, 64), (4, 1, 128), (3, 3, 128), (32, 2, 128), (6, 2, 16), (5, 5, 32), (9, 3, 48), (3, 1, 80), (8, 2, 96), (7, 1, 112)])
 def test_prompt_on_tcgen05(fmt, nh, nkv, hd):
     prompt_case(fmt, "bf16", nh, nkv, hd, [1], [1], form=2)
     prompt_case(fmt, "bf16", nh, nkv, hd, [17, 64], [17, 64], form=2)
@@ -80,10 +80,10 @@ def test_prompt_on_tcgen05(fmt, nh, nkv, hd):
 
 @pytest.mark.parametrize("splits", [1, 2, 3, 8])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 1, 128), (3, 1, 256)])
+@pytest.mark.parametrize("nh,nkv,hd", [(9, 3, 64), (4, 1, 128), (3, 1, 256), (3, 1, 48), (4, 2, 96)])
 def test_prompt_splits(splits, dtype, nh, nkv, hd):
     prompt_case("int8", dtype, nh, nkv, hd, TOTALS + [2500], NEWS + [70], splits=splits, form=1)
-    if dtype == "bf16" and hd in (64, 128):
+    if dtype == "bf16" and hd <= 128:
         for window in (0, 300):
             prompt_case("int8", dtype, nh, nkv, hd, TOTALS + [2500], NEWS + [70], splits=splits, form=2, window=window)
             prompt_case("fp8", dtype, nh, nkv, hd, [2500, 40], [3, 40], splits=splits, form=2, window=window)
