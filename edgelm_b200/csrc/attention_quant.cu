@@ -106,7 +106,9 @@ extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
   EL_REFUSE((uintptr_t)q % 16 == 0 && ldq % 4 == 0, "%s: query rows must start on a 16-byte boundary, a multiple of 4 numbers apart", who);
   EL_REFUSE((uintptr_t)out % 8 == 0 && ldo % 2 == 0, "%s: output rows must start on 8-byte boundaries", who);
   EL_REFUSE(form >= 0 && form <= 2, "%s: form %d", who, form);
-  const bool tc = form != 1 && err != nullptr && prefill_quant_tc_takes(q, ldq, out, ldo, dtype, hd);
+  // Sequences of one page stay on mma.sync: a block there starts sooner (us on mma.sync and tcgen05, 64 tokens: 9 heads of 64 on 3 5.6, 7.4; 16 of 128
+  // on 4 6.9, 9.9; 16 sequences of 12 heads of 96 on 4 8.2, 11.6; 128 tokens: 7.6, 7.6; 9.5, 10.2; 15.7, 18.4, and of 9 heads of 64 9.3, 8.2).
+  const bool taken = err != nullptr && prefill_quant_tc_takes(q, ldq, out, ldo, dtype, hd), tc = form == 2 ? taken : form == 0 && taken && max_keys > PAGE;
   EL_REFUSE(form != 2 || tc, "%s: these operands are not taken on tcgen05 (bfloat16, head size up to 128, 16-byte rows, an error word)", who);
   if (tc) {
     const int rc = launch_prefill_quant_tc(q, ldq, out, ldo, kcache, vcache, k_scale, v_scale, format, page_table, table_stride, n_pages, seq_slot, tile_seq,
