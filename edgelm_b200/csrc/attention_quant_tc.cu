@@ -20,7 +20,7 @@
 // Few rows over many keys (a short turn of a long conversation): a cluster of up to 8 blocks shares a row tile's key blocks, and the partial
 // results meet in distributed shared memory in a fixed order.
 // Bound by the softmax: a block of 128 keys takes 3,050 clocks, of them 630 to read and find the maxima, 440 at the exchange between a row's
-// threads, 1,280 for exponents, weights and sums, 305 waiting for S; the matrix products fill a quarter of it.  All 16 warps stand at the
+// threads, 1,280 for exponents, weights and sums, 305 waiting for S; the matrix products fill a sixth of it.  All 16 warps stand at the
 // same place; two teams of softmax warps on alternate blocks (28 warps, one block of keys behind the other) took 69.5 us for 68, and 88 for
 // 78 at a head size of 128: the registers of a thread then hold half of what they do now.  2,048 tokens of 32 heads of 64, e4m3: 68 us, 253
 // TFLOP/s by the products that the mask leaves; four turns of 65 to 701 tokens behind 1,501, 16 heads of 128 on 4, int8: 81 us.
