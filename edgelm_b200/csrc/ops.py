@@ -1547,6 +1547,9 @@ def softcap(z, cap):
 # with a float32 scale a row [pages, kv_heads, PAGE].  A row x is kept as scale = A / top and codes round(x * (top / A)) with
 # A = max(|x_i|, 2^-60) and top 127 (int8) or 448 (e4m3); a row with a number that is not finite has the scale NaN and codes of zero.
 
+_raw_stream = torch._C._cuda_getCurrentRawStream     # a device's index -> the current stream's handle
+_current_device = torch._C._cuda_getDevice
+
 QUANT_FORMATS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 QUANT_PREFILL_TILE = 128   # new tokens per tile of the prompt attention over the 8-bit cache
 QUANT_CLUSTER = 8          # blocks of a cluster in the decode attention; 16 clusters at most share a sequence (attention_quant_decode.cuh)
@@ -1580,17 +1583,18 @@ def _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what):
     if code is None or vcache.dtype != kcache.dtype:
         raise KernelError(f"{what}: the cache's codes must be int8 or float8_e4m3fn, keys and values alike")
     shape = kcache.shape
-    if len(shape) != 4 or shape[1:] != (nkv, PAGE, hd) or vcache.shape != shape:
+    n_pages = shape[0] if shape else 0
+    if shape != (n_pages, nkv, PAGE, hd) or vcache.shape != shape:
         raise KernelError(f"{what}: codes must be [pages, {nkv}, {PAGE}, {hd}]")
-    rows = shape[:3]
+    rows = (n_pages, nkv, PAGE)
     if k_scale.shape != rows or v_scale.shape != rows or not k_scale.dtype == v_scale.dtype == torch.float32:
         raise KernelError(f"{what}: scales must be float32 [pages, {nkv}, {PAGE}]")
     if not (kcache.is_contiguous() and vcache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise KernelError(f"{what}: the cache must be contiguous")
     device = kcache.get_device()
-    if device < 0 or device != torch._C._cuda_getDevice() or not device == vcache.get_device() == k_scale.get_device() == v_scale.get_device():
+    if device < 0 or device != _current_device() or not device == vcache.get_device() == k_scale.get_device() == v_scale.get_device():
         raise KernelError(f"{what}: the cache must lie on the current device")
-    return code, device, shape[0]
+    return code, device, n_pages
 
 
 def _quant_steps(page_table, tensors, device, what):
@@ -1629,9 +1633,6 @@ def _quant_rows(q, out, width, nh, hd, device, what):
     if q_shape[1] < width or o_shape[1] < nh * hd or q.get_device() != device or out.get_device() != device:
         raise KernelError(f"{what}: rows of {width} and {nh * hd} numbers on the cache's device are wanted")
     return qs[0], os[0], q_shape[0], o_shape[0]
-
-
-_raw_stream = torch._C._cuda_getCurrentRawStream     # a device's index -> the current stream's handle
 
 
 def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, kcache, vcache, k_scale, v_scale, nh, nkv, hd, err, q_out=None):

@@ -230,3 +230,33 @@ def test_query_rows_that_are_no_numbers_stay_to_themselves(fmt, dtype, form):
         ops.attn_decode_quantized(q.reshape(2, nh * hd), out.view(2, nh * hd), *cache_args(cache), table, i32(range(2)), pos, 2, nh, nkv, hd, 0.1)
         outs.append(out)
     assert torch.equal(outs[1].isnan().all(-1), hit[:2]) and torch.equal(outs[0][~hit[:2]], outs[1][~hit[:2]]) and bool(outs[0].isfinite().all())
+
+
+@pytest.mark.parametrize("nkv,hd", [(1, 256), (2, 128)])
+def test_offsets_beyond_32_bits(nkv, hd):
+    """A cache of more than 2^32 codes whose last pages are used: the same codes and outputs as in a small one."""
+    nh, totals, news = 4 * nkv, [200, 70], [200, 70]
+    pages = (1 << 32) // (nkv * 64 * hd) + 200
+    big = {n: torch.zeros((pages, nkv, 64, hd), dtype=torch.int8, device=DEV) for n in ("k", "v")} | {n: torch.zeros((pages, nkv, 64), device=DEV) for n in ("ks", "vs")}
+    small = {n: torch.zeros_like(t[:8]) for n, t in big.items()}
+    table = torch.tensor([[0, 3, 5, 1], [7, 2, 6, 4]], dtype=torch.int32, device=DEV)
+    qkv = torch.randn((sum(news), (nh + 2 * nkv) * hd), generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to(DEV)
+    pos, seq = i32([*range(200), *range(70)]), i32([0] * 200 + [1] * 70)
+    angles = torch.arange(256.0, device=DEV)[:, None] * 10000.0 ** (-torch.arange(0, hd, 2, device=DEV) / hd)
+    cos, sin, err, (tiles, n_tiles) = angles.cos().contiguous(), angles.sin().contiguous(), word(), tiles_of(totals, news)
+    got = []
+    for cache, where in ((small, table), (big, table + (pages - 8))):
+        q, kept = qkv.clone(), cache_args(cache)
+        ops.rope_quantize_append(q, pos, seq, i32([0, 1]), where, cos, sin, *kept, nh, nkv, hd, err)
+        rows = [torch.empty((270, nkv, hd), dtype=q.dtype, device=DEV) for _ in range(2)]
+        ops.quantized_rows(*kept, pos, seq, i32([0, 1]), where, *rows, err)
+        outs = []
+        for form in (0, 1):
+            outs.append(torch.empty((270, nh * hd), dtype=q.dtype, device=DEV))
+            ops.attn_prefill_quantized(q, outs[-1], *kept, where, i32([0, 1]), *tiles, n_tiles, nh, nkv, hd, 0.1, err=err, form=form, n_splits=2)
+        step = qkv[[5, 6]].contiguous()
+        outs.append(torch.empty((2, nh * hd), dtype=q.dtype, device=DEV))
+        ops.attn_decode_rope_quantized(step, outs[-1], *kept, where, i32([0, 1]), i32([200, 70]), cos, sin, 2, nh, nkv, hd, 0.1, err=err)
+        assert int(err) == 0
+        got.append([q, *rows, *outs] + [t[-8:].clone() for t in cache.values()])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and not any(bool(t[:-8].any()) for t in big.values())
