@@ -46,6 +46,13 @@ def load_engine(model, dtype="bfloat16", ctx=1024, slots=8, max_tokens=None, bat
     return Engine(m, max_tokens, max_step_tokens=batch, max_seqs=None, profile=profile, use_graphs=use_graphs, cache_format=cache_format)
 
 
+def _check_format(engine, cache_format):
+    if engine is not None and cache_format not in (None, engine.cache.format):
+        from .engine.engine import EngineError
+        raise EngineError(f"cache_format '{cache_format}' is asked for, but the engine's cache is kept in "
+                          f"{engine.cache.format or 'the compute dtype'}")
+
+
 def generate(model, prompts, n=64, temp=0.0, top_k=40, seed=42, stop=None, ignore_eos=False, dtype="bfloat16",
              ctx=1024, slots=8, engine=None, return_details=False, cache_format=None):
     """Generate up to `n` tokens for every prompt (lists of token ids).
@@ -53,8 +60,9 @@ def generate(model, prompts, n=64, temp=0.0, top_k=40, seed=42, stop=None, ignor
     `model` is a model folder; or pass a ready `engine`.  Options as edgelm's run command:
     temp (0 = greedy), top_k (40; <= 0 whole vocabulary), seed (42); `stop` defaults to the
     model's eos ids.  Prompts run in batches of at most `slots` sequences, one batch after
-    another.  `cache_format` as in `load_engine`.  Returns a list of token lists (or Generation records with return_details)."""
+    another.  `cache_format` as in `load_engine` (with a ready `engine`: its own, or None).  Returns a list of token lists (or Generation records with return_details)."""
     from .engine.generate import GenerationLoop
+    _check_format(engine, cache_format)
     eng = engine or load_engine(model, dtype=dtype, ctx=ctx, slots=slots, cache_format=cache_format)
     stop_ids = eng.plan.stop_token_ids if stop is None else stop
     loop = GenerationLoop(eng, SamplingParams(float(temp), int(top_k), int(seed)), max_new_tokens=n, stop_ids=stop_ids,
@@ -71,6 +79,7 @@ class Session:
     number of tokens in the cache."""
 
     def __init__(self, model, dtype="bfloat16", max_ctx=1024, max_batch=128, all_logits=False, profile=False, engine=None, cache_format=None):
+        _check_format(engine, cache_format)
         self.engine = engine or load_engine(model, dtype=dtype, ctx=max_ctx, slots=1, batch=max_batch, profile=profile, cache_format=cache_format)
         self.all_logits = all_logits
         self.slot = self.engine.open(1)[0]

@@ -2,9 +2,11 @@
 import pytest
 import torch
 
+import edgelm_b200
 import helpers as H
 from edgelm_b200.cache import CacheError, SequenceCache
 from edgelm_b200.config import ConfigError, config_class_for
+from edgelm_b200.engine.engine import EngineError
 from edgelm_b200.engine.model import DecoderModel
 from edgelm_b200.parts.base import KVNeed, NeedSet, StateNeed
 from edgelm_b200.presets import preset_config
@@ -81,3 +83,14 @@ def test_the_command_line_knows_the_formats(capsys):
     with pytest.raises(SystemExit):
         build_parser().parse_args(["run", "--cache", "int4"])
     assert H.TINY       # (the tiny models that the engine's tests run)
+
+
+@pytest.mark.parametrize("kept,asked", [(None, "int8"), ("int8", "fp8")])
+def test_a_ready_engine_with_another_format_is_refused(kept, asked):
+    class Ready:
+        class cache:
+            format = kept
+    with pytest.raises(EngineError, match=asked):
+        edgelm_b200.Session("nowhere", engine=Ready(), cache_format=asked)
+    with pytest.raises(EngineError, match=asked):
+        edgelm_b200.generate("nowhere", [[1]], engine=Ready(), cache_format=asked)
