@@ -56,7 +56,7 @@ template <int HD> struct QtSizes {
   static constexpr int BARS = ROW_SUM + QT_GROUPS * QT_ROWS * 4;
   static constexpr int N_BARS = 1 + 2 + 2 + 2 * KS + 2 * VS + 2 + 2 + 2 + 4 + 1;
   static constexpr int needed = 1024 + BARS + N_BARS * 8 + 8;                     // (behind the barriers: the tensor memory's address and the abort flag)
-  // one block an SM: two blocks of different clusters on one SM could each hold the tensor memory that the other's cluster waits for
+  // one block an SM, whose tensor memory has room for one: a second would wait there for the first instead of going to the next free SM
   static constexpr int smem = needed > 114 * 1024 ? needed : 114 * 1024;
   static_assert(CODES % 16 == 0 && KEY_DATA % 16 == 0 && BARS % 8 == 0, "alignment");
   static_assert(2 * (smem + 1024) > 228 * 1024, "one block an SM");
@@ -582,11 +582,14 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
 
 template <int HD, int FMT>
 static int launch_quant_tc(const QuantTcArgs& a, int n_tiles, int n_splits, cudaStream_t stream) {
-  constexpr int smem = QtSizes<HD>::smem;
-  static_assert(smem <= 227 * 1024, "shared memory");
+  // A cluster's blocks wait for one another with their tensor memory in hand.  They take all of an SM's shared memory, so that no block of
+  // another kernel's cluster (another stream's matrix product) can hold the tensor memory that one of them waits for and wait for another.
+  constexpr int all = 227 * 1024;
+  static_assert(QtSizes<HD>::smem <= all, "shared memory");
+  const int smem = n_splits > 1 ? all : QtSizes<HD>::smem;
   auto kern = attn_prefill_quant_tc_kernel<HD, FMT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  EL_REFUSE(e == cudaSuccess, "attn_prefill_quantized: %d bytes of shared memory refused: %s", smem, cudaGetErrorString(e));
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, all);
+  EL_REFUSE(e == cudaSuccess, "attn_prefill_quantized: %d bytes of shared memory refused: %s", all, cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n_splits, a.nkv, n_tiles * a.blocks_per_tile);
   cfg.blockDim = dim3(QT_THREADS);
