@@ -1747,8 +1747,8 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     """`attn_prefill` over the 8-bit cache: causal attention of new tokens (any number per sequence), as tiles of at most
     QUANT_PREFILL_TILE consecutive tokens of one sequence; the tokens' own keys and values are in the cache.  `max_keys`: the longest
     sequence's keys, if the caller knows them (0: the page table's width), by which the blocks that share keys are counted.
-    `form`: 0 on tcgen05 where it takes the operands (bfloat16, head size up to 128, 16-byte rows, with the error word), else on mma.sync;
-    1 on mma.sync; 2 on tcgen05.  `n_splits`: blocks that share a row tile's keys, 1 to 8 (None: by sizes)."""
+    `form`: 0 on tcgen05 where it takes the operands (bfloat16, head size up to 128, 16-byte rows, with the error word) and `max_keys` is more
+    than a page, else on mma.sync; 1 on mma.sync; 2 on tcgen05.  `n_splits`: blocks that share a row tile's keys, 1 to 8 (None: by sizes)."""
     what = "attn_prefill_quantized"
     _heads(nh, nkv, hd, what)
     code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
