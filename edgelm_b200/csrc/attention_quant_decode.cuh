@@ -371,14 +371,13 @@ attn_decode_quant_kernel(const QuantDecodeArgs p) {
           mx[h] = fmaxf(mx[h], fmaxf(x[mt][0][h], x[mt][1][h]));
         }
       }
-      float bias[HC], fold[HC];
+      float ref[HC], fold[HC];
 #pragma unroll
       for (int h = 0; h < HC; ++h) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], off));   // over the lanes that hold the other keys of the same heads
-        const float ref = mx[h] == -CUDART_INF_F ? 0.f : mx[h];   // (no score above minus infinity yet)
-        fold[h] = aq_exp2(m[h] - ref);
-        bias[h] = AQ_LIFT - ref;
+        ref[h] = mx[h] == -CUDART_INF_F ? 0.f : mx[h];   // (no score above minus infinity yet)
+        fold[h] = aq_exp2(m[h] - ref[h]);
         m[h] = mx[h];
         l[h] *= fold[h];
       }
@@ -399,7 +398,7 @@ attn_decode_quant_kernel(const QuantDecodeArgs p) {
         float wa[2] = {0.f, 0.f}, wb[2] = {0.f, 0.f};     // (f and 2^-e of a key that is not seen are zero, and so is its weight)
 #pragma unroll
         for (int h = 0; h < HC; ++h) {
-          const float ta = aq_exp2(x[mt][0][h] + bias[h]), tb = aq_exp2(x[mt][1][h] + bias[h]);
+          const float ta = aq_exp2(x[mt][0][h] - ref[h] + AQ_LIFT), tb = aq_exp2(x[mt][1][h] - ref[h] + AQ_LIFT);
           l[h] = fmaf(ta, sa.y, fmaf(tb, sb.y, l[h]));
           wa[h] = ta * sa.x;
           wb[h] = tb * sb.x;

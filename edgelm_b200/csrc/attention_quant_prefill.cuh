@@ -239,7 +239,17 @@ attn_prefill_quant_kernel(const QuantPrefillArgs p) {
       mb = xb;
       la *= fa;
       lb *= fb;
-      const float ba = AQ_LIFT - ref_a, bb = AQ_LIFT - ref_b;
+      float ba = AQ_LIFT - ref_a, bb = AQ_LIFT - ref_b;
+      if (fmaxf(fabsf(ref_a), fabsf(ref_b)) > AQ_FAR) {
+        ba = bb = AQ_LIFT;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          s[nt][0] -= ref_a;
+          s[nt][1] -= ref_a;
+          s[nt][2] -= ref_b;
+          s[nt][3] -= ref_b;
+        }
+      }
       uint32_t w[TERMS][NT][2];      // the weights as the A operand: rows gid and gid + 8, keys 2 tig and the next of every 8
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {

@@ -434,7 +434,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       float rescale = 1.f;
       if (j == 0) {
         m = mx;
-      } else if (mx > m + QT_LAZY) {
+      } else if (mx - m > QT_LAZY) {              // (a difference: far from zero m + 8 may be m, or m + 16)
         rescale = aq_exp2(m - mx);                 // (0 if the row has seen no key so far)
         m = mx;
         l *= rescale;
@@ -454,7 +454,15 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
           qt_tmem_st8(o_addr, o);
         }
       }
-      const float bias = AQ_LIFT - (m == -CUDART_INF_F ? 0.f : m);
+      const float reference = m == -CUDART_INF_F ? 0.f : m;
+      float bias = AQ_LIFT - reference;
+      if (fabsf(reference) > AQ_FAR) {             // (attention_quant.cuh; x - M as it was rounded for the maximum)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], f, e) - reference;
+        f = 1.f;
+        e = 0.f;
+        bias = AQ_LIFT;
+      }
       const uint64_t f2 = qt_pair(f, f), bias2 = qt_pair(e + bias, e + bias);
       uint64_t sum0 = 0, sum1 = 0;
       if (group.w == 0.f) {
