@@ -67,10 +67,11 @@ __device__ __forceinline__ ValueScale value_scale(float v) {
   return {(float)(b - 127), v * undo * AQ_OPERAND, undo};
 }
 
-// The power of two that brings a query row with this largest magnitude into [2^12, 2^13), and what undoes it.  (Rows that are not
-// finite stay so; rows of zeros, or under 2^-100, keep a factor whose inverse is a number.)
+// The power of two that brings a query row with this largest magnitude into [2^12, 2^13).  (Rows that are not finite stay so; rows of
+// zeros, or under 2^-100, keep a factor whose inverse is a number.)  Its inverse times the scores' scale is the row's factor, which a key's
+// scale joins before the product does: scores are numbers as long as they, and that factor times that scale, are within float32.
 __device__ __forceinline__ float query_lift(uint32_t largest_bits) {
-  const int e = min(max((int)(largest_bits >> 23), 27), 227) - 127;    // floor(log2), held to -100 .. 100
+  const int e = min(max((int)(largest_bits >> 23), 27), 254) - 127;    // floor(log2), held to -100 .. 127
   return __uint_as_float((uint32_t)(AQ_QUERY_EXP - e + 127) << 23);
 }
 

@@ -3,7 +3,7 @@
 // A block takes 64 (token, query head) rows of one kv head, token-major, so that all query heads of a kv head share what is read; a
 // warp owns 16 of them.  A tile of keys (64, from head size 144 on 32) arrives as four bulk copies of codes and scales into a ring
 // of two stages; the block's threads turn it ONCE into float16 rows (padded by 16 bytes, so that ldmatrix reads hit distinct
-// banks) and per key {u log2(e) scale, e, f, 2^-e} (attention_quant.cuh), one tile ahead of the one that is being multiplied.  A tile's
+// banks) and per key {u, e, f, 2^-e} (attention_quant.cuh), one tile ahead of the one that is being multiplied.  A tile's
 // weighted values are a sum of their own that joins the running one by a rounded multiply-add.
 //
 // Few rows over many keys (a short turn of a long conversation): a cluster of up to 8 blocks shares a row tile's keys, and the
@@ -133,7 +133,7 @@ attn_prefill_quant_kernel(const QuantPrefillArgs p) {
       *reinterpret_cast<uint2*>(dst + 8 * i) = make_uint2(lo, hi);
       if (TERMS == 2) *reinterpret_cast<uint2*>(dst + QP_ROWS * PITCH + 8 * i) = make_uint2(aq_rest(x0, x1, lo), aq_rest(x2, x3, hi));
     }
-    if ((lane & 1) == 0) factors[row] = 1.0f / lift;
+    if ((lane & 1) == 0) factors[row] = 1.0f / lift * (p.scale * AQ_LOG2E);
   }
   __syncwarp();
   const int ra = warp * 16 + gid, rb = ra + 8;             // this lane's rows
@@ -162,7 +162,7 @@ attn_prefill_quant_kernel(const QuantPrefillArgs p) {
     if (threadIdx.x < KT) {
       const float* u = reinterpret_cast<const float*>(src + 2 * KT * HD);
       const ValueScale s = value_scale(u[KT + threadIdx.x]);
-      key_data[b * KT + threadIdx.x] = make_float4(u[threadIdx.x] * (p.scale * AQ_LOG2E), s.e, s.f, s.undo);
+      key_data[b * KT + threadIdx.x] = make_float4(u[threadIdx.x], s.e, s.f, s.undo);
     }
   };
   float o[2 * HDT][4];

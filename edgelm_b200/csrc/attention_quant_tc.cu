@@ -47,8 +47,8 @@ template <int HD> struct QtSizes {
   static constexpr int KC = (HD + 63) / 64;                   // tiles of 64 dims (what lies behind a row's end in the last is not read, or its products are not)
   static constexpr int KS = 2, VS = KC == 1 ? 2 : 1;          // stages of keys and values (shared memory has room for one of values at 128)
   static constexpr int CODES = QT_KEYS * (2 * HD + 8);        // a stage: key codes, value codes, key scales, value scales
-  static constexpr int KEY_DATA = QT_GROUPS * 16 + 4 * QT_KEYS * 4;   // a block's groups {2^k scale log2(e), e, 2^-e, slow}, and of every key (where
-                                                                      // its group is slow) u scale log2(e), e, f 2^-40, 2^-e; four blocks' worth
+  static constexpr int KEY_DATA = QT_GROUPS * 16 + 4 * QT_KEYS * 4;   // a block's groups {2^k, e, 2^-e, slow}, and of every key (where
+                                                                      // its group is slow) u, e, f 2^-40, 2^-e; four blocks' worth
   // where things lie, from a 1,024-byte boundary on
   static constexpr int KEYS = KC * QT_TILE, VALUES = KEYS + KS * KC * QT_TILE, CODES_AT = VALUES + VS * KC * QT_TILE, KEY_DATA_AT = CODES_AT + 2 * CODES;
   static constexpr int ROW_MAX = KEY_DATA_AT + 4 * KEY_DATA;                      // [block & 1][group][128 rows]
@@ -283,12 +283,12 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       const float un_k = __uint_as_float((uint32_t)(254 - min(umax, 253)) << 23), un_e = __uint_as_float((uint32_t)(254 - min(vmax, 253)) << 23);
       float* kd = reinterpret_cast<float*>(key_data + (j & 3) * Z::KEY_DATA);
       if (lane == 0)
-        reinterpret_cast<float4*>(kd)[cw] = make_float4(1.0f / un_k * scale2, (float)(min(vmax, 253) - 127), un_e, slow ? 1.f : 0.f);
+        reinterpret_cast<float4*>(kd)[cw] = make_float4(1.0f / un_k, (float)(min(vmax, 253) - 127), un_e, slow ? 1.f : 0.f);
       float mk = fine ? u * un_k : CUDART_NAN_F, mv = fine ? v * un_e : 0.f;
       if (slow) {
         const ValueScale vsc = value_scale(fine ? v : 0.f);
         kd += QT_GROUPS * 4 + cw * 32 + lane;
-        kd[0] = fine ? u * scale2 : CUDART_NAN_F;
+        kd[0] = fine ? u : CUDART_NAN_F;
         kd[QT_KEYS] = vsc.e;
         kd[2 * QT_KEYS] = vsc.f * (QT_OPERAND / AQ_OPERAND);
         kd[3 * QT_KEYS] = vsc.undo;
@@ -366,7 +366,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
       most = max(max(at[row], at[QT_ROWS + row]), max(at[2 * QT_ROWS + row], at[3 * QT_ROWS + row]));
       meet();                                      // (all have read, before the maxima are written over)
       const float lift = query_lift(most);
-      qf = 1.0f / lift;
+      qf = 1.0f / lift * scale2;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -403,7 +403,7 @@ attn_prefill_quant_tc_kernel(const QuantTcArgs a) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             const ulonglong2 u = kd[i / 4], o = kd[32 + i / 4];
-            const float2 y = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i], x[i + 1]), u.x), f2, o.x)), z = qt_unpair(qt_fma2(qt_mul2(qt_pair(x[i + 2], x[i + 3]), u.y), f2, o.y));
+            const float2 y = qt_unpair(qt_fma2(qt_pair(x[i], x[i + 1]), qt_mul2(u.x, f2), o.x)), z = qt_unpair(qt_fma2(qt_pair(x[i + 2], x[i + 3]), qt_mul2(u.y, f2), o.y));
             x[i] = y.x;
             x[i + 1] = y.y;
             x[i + 2] = z.x;

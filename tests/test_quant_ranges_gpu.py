@@ -70,3 +70,41 @@ def test_scores_far_from_zero(kernel, dtype, nh, nkv, hd, splits, power):
         cache["ks"].mul_(2.0 ** (power - torch.randint(0, 13 if per_key else 6, shape, generator=g)).to(DEV))
         q = torch.randn((n, nh, hd), generator=g).to(DTYPES[dtype]).to(DEV)
         check_one_key_takes_all(kernel, q, cache, table, total, nh, nkv, hd, 1 / math.sqrt(hd), splits)
+
+
+@pytest.mark.parametrize("power", [-90, -40, 60, 101, 104, 110, 118])
+@pytest.mark.parametrize("kernel,dtype,nh,nkv,hd,splits", KERNELS)
+def test_queries_of_any_size(kernel, dtype, nh, nkv, hd, splits, power):
+    """Queries 2^power times as large under a scale 2^-power times as large are the same scores: the same bits.  (tcgen05: also where
+    scales go into the scores a key at a time.)"""
+    total, n = 300, 70
+    for fmt, per_key in (("int8", False), ("fp8", True)):
+        cache, table = ref.make_cache(fmt, nkv, hd, [total], DEV, 3)
+        g = torch.Generator().manual_seed(5)
+        if per_key:
+            cache["ks"].mul_(2.0 ** -torch.randint(0, 13, cache["ks"].shape, generator=g).to(DEV))
+        q, scale = torch.randn((n, nh, hd), generator=g).to(DTYPES[dtype]).to(DEV), 1 / math.sqrt(hd)
+        args = (cache, table, total, nh, nkv, hd)
+        assert torch.equal(attend(kernel, q, *args, scale, splits), attend(kernel, q * 2.0 ** power, *args, scale * 2.0 ** -power, splits))
+
+
+@pytest.mark.parametrize("power", [100, 101, 104, 110])
+@pytest.mark.parametrize("kernel,dtype,nh,nkv,hd,splits", KERNELS)
+def test_queries_as_large_as_float32_holds(kernel, dtype, nh, nkv, hd, splits, power):
+    """.. and under the usual scale they are numbers too: every row the value of one key."""
+    total, n = 300, 70
+    cache, table = ref.make_cache("int8", nkv, hd, [total], DEV, 3)
+    q = torch.randn((n, nh, hd), generator=torch.Generator().manual_seed(5)).to(DTYPES[dtype]).to(DEV) * 2.0 ** power
+    check_one_key_takes_all(kernel, q, cache, table, total, nh, nkv, hd, 1 / math.sqrt(hd), splits)
+
+
+@pytest.mark.parametrize("kernel,dtype,nh,nkv,hd,splits", KERNELS)
+def test_large_keys_under_small_queries(kernel, dtype, nh, nkv, hd, splits):
+    """Keys of up to 2^118 under queries of about 2^-98, each key with a scale of its own: that scale times the codes' product is beyond
+    float32 before the query's factor joins them, the score is not."""
+    total, n = 300, 70
+    cache, table = ref.make_cache("fp8", nkv, hd, [total], DEV, 3)
+    g = torch.Generator().manual_seed(5)
+    cache["ks"].mul_(2.0 ** (115 - torch.randint(0, 13, cache["ks"].shape, generator=g)).to(DEV))
+    q = torch.randn((n, nh, hd), generator=g).to(DTYPES[dtype]).to(DEV) * 2.0 ** -98
+    check_one_key_takes_all(kernel, q, cache, table, total, nh, nkv, hd, 1 / math.sqrt(hd), splits)
