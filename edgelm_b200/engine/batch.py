@@ -92,10 +92,17 @@ class StepContext:
         return list(self._seq_pos0)
 
     @property
+    def keys_bound(self):
+        """At least the keys that the step's longest sequence has when the step is done: their pages rounded up to a power of two,
+        in tokens.  What a part may choose launches by where a captured graph of the step is keyed by it."""
+        pages = -(-max(p + n for p, n in zip(self._seq_pos0, self._seq_ntok)) // ops.PAGE)
+        return ops.PAGE << (pages - 1).bit_length()
+
+    @property
     def all_fresh(self):
         """Whether every sequence of the step starts at its position 0 (prompts that bring their first tokens): such a
-        step sees no key or state but its own.  A part may take another path then; with `all_single` it is one of the
-        two facts about a step's positions that a captured graph of the step is keyed by."""
+        step sees no key or state but its own.  A part may take another path then; with `all_single` (and, over a cache kept
+        in an 8-bit format, `keys_bound`) it is what a captured graph of the step is keyed by of the step's positions."""
         return not any(self._seq_pos0)
 
     def decode_splits(self, n_kv_heads, resident=None):

@@ -107,7 +107,7 @@ class Engine:
         self.sampler = DeviceSampler(self.cache.n_slots, self.device)
         self.use_graphs = bool(use_graphs) and not profile and model.graph_safe
         self._graphs = {}
-        self._step_graphs = {}     # shape of a step (tokens per sequence, wanted rows) -> captured forward
+        self._step_graphs = {}     # shape of a step (tokens per sequence, wanted rows; see `_replay_step`) -> captured forward
         self._step_seen = {}
         self.steps_run = 0
         self.h2d_bytes_last = 0
@@ -259,8 +259,10 @@ class Engine:
         self.steps_run += 1
         return len(want_rows)
 
-    # A step's launches depend on its shape only (tokens per sequence, number of wanted rows): ids,
-    # positions, page tables, tiles and wanted rows are data in the fixed metadata buffer.  So a
+    # A step's launches depend on its shape (tokens per sequence, number of wanted rows), on whether all its
+    # sequences start with it, and, over an 8-bit cache, on `keys_bound`; ids, positions, page tables, tiles and
+    # wanted rows are data in the fixed metadata buffer.  (Attention over other caches on mma.sync takes the step's
+    # keys as a hint, and a replayed step keeps that of the one it was captured from.)  So a
     # shape that comes back is replayed from a CUDA graph, which removes the host's launch work
     # (a prompt step is otherwise bound by it).  Captured at a shape's second appearance; the
     # graph writes logits into a buffer of its own, copied out after the replay.
@@ -278,6 +280,8 @@ class Engine:
         # (a part may run a step of first tokens another way, `StepContext.all_fresh`: such a step and one of the same shape
         # that goes on from earlier tokens are two graphs)
         key = (shape, n_want) if ctx.all_fresh else (shape, n_want, "continued")
+        if self.cache.format is not None:
+            key += (ctx.keys_bound,)
         g = self._step_graphs.get(key)
         if g is None:
             self._step_seen[key] = self._step_seen.get(key, 0) + 1

@@ -171,7 +171,7 @@ class Attention(Part):
         tiles = ctx.tiles(ops.QUANT_PREFILL_TILE)
         with ctx.prof("attn_prefill"):
             ops.attn_prefill_quantized(qkv, a, *kept, table, ctx.seq_index, tiles.seq, tiles.tok0, tiles.ntok, tiles.pos0, tiles.count, self.nh, self.nkv,
-                                       self.hd, self.scale, err=ctx.err, window=self.window, max_keys=max(p + n for p, n in zip(ctx.seq_first_positions, ctx.seq_lengths)))
+                                       self.hd, self.scale, err=ctx.err, window=self.window, max_keys=ctx.keys_bound)
 
     def forward(self, ctx, h, x, cache):
         T = h.shape[0]
