@@ -1747,6 +1747,7 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     """`attn_prefill` over the 8-bit cache: causal attention of new tokens (any number per sequence), as tiles of at most
     QUANT_PREFILL_TILE consecutive tokens of one sequence; the tokens' own keys and values are in the cache.  `max_keys`: the longest
     sequence's keys, if the caller knows them (0: the page table's width), by which the blocks that share keys are counted.
+    More blocks than a grid takes go in several launches.
     `form`: 0 on tcgen05 where it takes the operands (bfloat16, head size up to 128, 16-byte rows, with the error word) and `max_keys` is more
     than a page, else on mma.sync; 1 on mma.sync; 2 on tcgen05.  `n_splits`: blocks that share a row tile's keys, 1 to 8 (None: by sizes)."""
     what = "attn_prefill_quantized"
@@ -1762,7 +1763,12 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     keys = max_keys or page_table.shape[1] * PAGE
     if window > 0:
         keys = min(keys, window + most)
-    _call_packed("edgelm_attn_prefill_quantized", 1 if n_tiles else 0, _QUANT_PREFILL,
-        qkv.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
-        tile_seq.data_ptr(), tile_tok0.data_ptr(), tile_ntok.data_ptr(), tile_pos0.data_ptr(), err.data_ptr() if err is not None else 0, _raw_stream(device),
-        ldq, ldo, _dt(qkv), code, pitch, n_pages, n_tiles, most, nh, nkv, hd, n_splits or 0, keys, window, form, scale)
+    # (65,535 blocks along the grid's tiles; a block has at least 64 of a tile's rows of a kv head)
+    at_a_time = max(1, 65535 // max(1, -(-most * (nh // nkv) // 64)))
+    for first in range(0, n_tiles, at_a_time) if n_tiles > at_a_time else (0,):
+        tiles, ahead = min(at_a_time, n_tiles - first), 4 * first
+        _call_packed("edgelm_attn_prefill_quantized", 1 if n_tiles else 0, _QUANT_PREFILL,
+            qkv.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
+            tile_seq.data_ptr() + ahead, tile_tok0.data_ptr() + ahead, tile_ntok.data_ptr() + ahead, tile_pos0.data_ptr() + ahead,
+            err.data_ptr() if err is not None else 0, _raw_stream(device), ldq, ldo, _dt(qkv), code, pitch, n_pages, tiles, most, nh, nkv, hd, n_splits or 0, keys,
+            window, form, scale)
