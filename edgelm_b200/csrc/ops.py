@@ -1743,11 +1743,12 @@ def attn_decode_rope_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_
 
 
 def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok, tile_pos0, n_tiles, nh, nkv,
-                           hd, scale, err=None, window=0, max_keys=0, n_splits=None, form=0):
+                           hd, scale, err=None, window=0, max_keys=0, n_splits=None, form=0, max_tile_tokens=0):
     """`attn_prefill` over the 8-bit cache: causal attention of new tokens (any number per sequence), as tiles of at most
     QUANT_PREFILL_TILE consecutive tokens of one sequence; the tokens' own keys and values are in the cache.  `max_keys`: the longest
     sequence's keys, if the caller knows them (0: the page table's width), by which the blocks that share keys are counted.
-    More blocks than a grid takes go in several launches.
+    `max_tile_tokens`: the longest tile's tokens, if the caller knows them (0: QUANT_PREFILL_TILE, or all rows if they are fewer), by which the
+    blocks of a tile are counted: what a longer tile has more is not computed.  More blocks than a grid takes go in several launches.
     `form`: 0 on tcgen05 where it takes the operands (bfloat16, head size up to 128, 16-byte rows, with the error word) and `max_keys` is more
     than a page, else on mma.sync; 1 on mma.sync; 2 on tcgen05.  `n_splits`: blocks that share a row tile's keys, 1 to 8 (None: by sizes)."""
     what = "attn_prefill_quantized"
@@ -1759,7 +1760,7 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     wanted = ((seq_slot, 0), (tile_seq, n_tiles), (tile_tok0, n_tiles), (tile_ntok, n_tiles), (tile_pos0, n_tiles))
     pitch = _quant_steps(page_table, wanted if err is None else wanted + ((err, 1),), device, what)
     window = int(window or 0)
-    most = max(1, min(QUANT_PREFILL_TILE, rows_q))
+    most = max_tile_tokens or max(1, min(QUANT_PREFILL_TILE, rows_q))
     keys = max_keys or page_table.shape[1] * PAGE
     if window > 0:
         keys = min(keys, window + most)

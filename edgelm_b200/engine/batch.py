@@ -92,6 +92,11 @@ class StepContext:
         return list(self._seq_pos0)
 
     @property
+    def most_new_tokens(self):
+        """The tokens that the sequence with the most of them brings in this step."""
+        return max(self._seq_ntok)
+
+    @property
     def keys_bound(self):
         """At least the keys that the step's longest sequence has when the step is done: their pages rounded up to a power of two,
         in tokens.  What a part may choose launches by where a captured graph of the step is keyed by it."""

@@ -171,7 +171,8 @@ class Attention(Part):
         tiles = ctx.tiles(ops.QUANT_PREFILL_TILE)
         with ctx.prof("attn_prefill"):
             ops.attn_prefill_quantized(qkv, a, *kept, table, ctx.seq_index, tiles.seq, tiles.tok0, tiles.ntok, tiles.pos0, tiles.count, self.nh, self.nkv,
-                                       self.hd, self.scale, err=ctx.err, window=self.window, max_keys=ctx.keys_bound)
+                                       self.hd, self.scale, err=ctx.err, window=self.window, max_keys=ctx.keys_bound,
+                                       max_tile_tokens=min(ops.QUANT_PREFILL_TILE, ctx.most_new_tokens))
 
     def forward(self, ctx, h, x, cache):
         T = h.shape[0]

@@ -27,3 +27,37 @@ def test_more_tiles_than_one_grid_takes(dtype, form):
         part = [t[a:a + 1000].contiguous() for t in tiles]
         call(pieces, part, part[0].numel())
     assert int(err) == 0 and torch.equal(out, pieces) and bool(out.isfinite().all()) and bool((out != 0).any(1).all())
+
+
+@pytest.mark.parametrize("dtype,form", [(torch.bfloat16, 2), (torch.bfloat16, 1), (torch.float32, 1)])
+def test_the_longest_tile_as_the_caller_knows_it(dtype, form):
+    """Blocks counted by the step's longest tile give what blocks for whole tiles give; a number that no tile has is refused."""
+    nh, nkv, hd, news = 9, 3, 64, [17, 3, 1, 17, 9]
+    totals = [400, 3, 200, 64, 130]
+    cache, table = ref.make_cache("fp8", nkv, hd, totals, DEV, 3)
+    q = torch.randn((sum(news) + 90, nh * hd), generator=torch.Generator().manual_seed(4)).to(dtype).to(DEV)
+    tiles, n_tiles = tiles_of(totals, news)
+    outs, err = [], word()
+    for window in (0, 100):
+        for most in (0, 17, 20, 128):
+            outs.append(torch.zeros_like(q))
+            ops.attn_prefill_quantized(q, outs[-1], *cache_args(cache), table, i32(range(5)), *tiles, n_tiles, nh, nkv, hd, 0.125, err=err, n_splits=2, form=form,
+                                       window=window, max_tile_tokens=most)
+            assert torch.equal(outs[-1], outs[len(outs) // 5 * 4])
+    assert int(err) == 0 and bool((outs[0][sum(news):] == 0).all())
+    for most in (-1, 129):
+        with pytest.raises(ops.KernelError, match="1 to 128"):
+            ops.attn_prefill_quantized(q, outs[0], *cache_args(cache), table, i32(range(5)), *tiles, n_tiles, nh, nkv, hd, 0.125, max_tile_tokens=most)
+
+
+def test_an_engine_says_how_long_its_tiles_are(tmp_path, monkeypatch):
+    from edgelm_b200.engine.engine import Engine, StepEntry
+    eng = Engine.from_dir(H.make_model_dir(tmp_path, "tiny_d"), dtype="bfloat16", max_tokens=4096, cache_format="int8", use_graphs=False)
+    told, real = [], ops.attn_prefill_quantized
+    monkeypatch.setattr(ops, "attn_prefill_quantized", lambda *a, **kw: (told.append(kw["max_tile_tokens"]), real(*a, **kw)))
+    slots = eng.open(8)
+    for news in ([17] * 8, [1] * 7 + [5], [300] + [2] * 7):
+        told.clear()
+        eng.step([StepEntry(s, H.tokens_for("tiny_d", n, i), [n - 1]) for i, (s, n) in enumerate(zip(slots, news))])
+        assert told and set(told) == {min(128, max(news))}
+    eng.check_device_errors()
