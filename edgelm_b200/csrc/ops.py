@@ -1598,15 +1598,16 @@ def _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what):
 
 
 def _quant_steps(page_table, tensors, device, what):
-    """Checks the page table and the (tensor, least count) pairs; the table's pitch."""
-    stride = page_table.stride()
-    if len(stride) != 2 or stride[1] != 1 or page_table.dtype != torch.int32 or page_table.get_device() != device:
+    """Checks the page table and the (tensor, least count) pairs; the table as the kernels read it, and its pitch: the kernels look up
+    no page behind the pitch, so it has to be the width, and a view whose rows lie otherwise is laid out anew."""
+    stride, shape = page_table.stride(), page_table.shape
+    if len(stride) != 2 or (stride[1] != 1 and shape[1] > 1) or page_table.dtype != torch.int32 or page_table.get_device() != device:
         raise KernelError(f"{what}: the page table must be int32 rows on the cache's device")
     for t, n in tensors:
         if t.dtype != torch.int32 or t.get_device() != device or not t.is_contiguous() or t.numel() < n:
             raise KernelError(f"{what}: positions, indices, tiles and the error word must be contiguous int32 tensors on the cache's device, one number each "
                               f"per token, sequence or tile (at least {n} here)")
-    return stride[0]
+    return page_table if stride[0] == shape[1] or shape[0] == 1 else page_table.contiguous(), shape[1]
 
 
 def _quant_tables(cos, sin, hd, device, what):
@@ -1649,7 +1650,7 @@ def rope_quantize_append(qkv, tok_pos, tok_seq, seq_slot, page_table, cos, sin, 
     if q_out is not None and (q_out.shape != (T, nh * hd) or q_out.dtype != qkv.dtype or not q_out.is_contiguous() or q_out.get_device() != device):
         raise KernelError(f"{what}: q_out must be contiguous rows of {nh * hd} numbers, one per token, of the projections' type")
     max_pos = _quant_tables(cos, sin, hd, device, what)
-    pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
+    page_table, pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
     _call_packed("edgelm_rope_quantize_append", 1 if T else 0, _QUANT_APPEND,
         qkv.data_ptr(), q_out.data_ptr() if q_out is not None else 0, tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(),
         cos.data_ptr(), sin.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), err.data_ptr(), _raw_stream(device),
@@ -1668,7 +1669,7 @@ def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot,
     code, device, n_pages = _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what)
     if not keys.get_device() == values.get_device() == device:
         raise KernelError(f"{what}: rows must lie on the cache's device")
-    pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
+    page_table, pitch = _quant_steps(page_table, ((tok_pos, T), (tok_seq, T), (seq_slot, 0), (err, 1)), device, what)
     _call_packed("edgelm_quantized_rows", 1 if T else 0, _QUANT_ROWS,
         kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(),
         page_table.data_ptr(), keys.data_ptr(), values.data_ptr(), err.data_ptr(), _raw_stream(device), code, _dt(keys), pitch, n_pages, T, nkv, hd)
@@ -1699,7 +1700,7 @@ def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_
     ldq, ldo, rows_q, rows_out = _quant_rows(q, out, nh * hd if cos is None else (nh + 2 * nkv) * hd, nh, hd, device, what)
     if n_seqs < 0 or rows_q < n_seqs or rows_out < n_seqs:
         raise KernelError(f"{what}: a row of queries and of outputs per sequence is wanted")
-    pitch = _quant_steps(page_table, ((seq_slot, n_seqs), (seq_pos, n_seqs)) if err is None else ((seq_slot, n_seqs), (seq_pos, n_seqs), (err, 1)), device, what)
+    table, pitch = _quant_steps(page_table, ((seq_slot, n_seqs), (seq_pos, n_seqs)) if err is None else ((seq_slot, n_seqs), (seq_pos, n_seqs), (err, 1)), device, what)
     window = int(window or 0)
     if n_splits is None:
         keys = page_table.shape[1] * PAGE
@@ -1717,9 +1718,9 @@ def _attn_decode_quantized(what, q, out, kcache, vcache, k_scale, v_scale, page_
         max_pos = _quant_tables(cos, sin, hd, device, what)
         cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
     _call_packed("edgelm_attn_decode_quantized", (2 if part else 1) if n_seqs else 0, _QUANT_DECODE,
-        q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
+        q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(), seq_slot.data_ptr(),
         seq_pos.data_ptr(), cos_ptr, sin_ptr, err.data_ptr() if err is not None else 0, part, _raw_stream(device), ldq, ldo, _dt(q), code, pitch, n_pages, max_pos,
-        n_seqs, nh, nkv, hd, n_splits, window, 1 if meta_ready else 0, scale)
+        n_seqs, nh, nkv, hd, n_splits, window, 1 if meta_ready and table is page_table else 0, scale)     # (a table laid out just now is not that old)
 
 
 def attn_decode_quantized(q, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, n_seqs, nh, nkv, hd, scale, n_splits=None,
@@ -1758,7 +1759,7 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     if rows_q != rows_out:
         raise KernelError(f"{what}: a row of outputs per row of queries is wanted")
     wanted = ((seq_slot, 0), (tile_seq, n_tiles), (tile_tok0, n_tiles), (tile_ntok, n_tiles), (tile_pos0, n_tiles))
-    pitch = _quant_steps(page_table, wanted if err is None else wanted + ((err, 1),), device, what)
+    page_table, pitch = _quant_steps(page_table, wanted if err is None else wanted + ((err, 1),), device, what)
     window = int(window or 0)
     most = max_tile_tokens or max(1, min(QUANT_PREFILL_TILE, rows_q))
     keys = max_keys or page_table.shape[1] * PAGE
