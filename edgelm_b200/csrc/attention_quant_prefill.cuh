@@ -174,7 +174,8 @@ attn_prefill_quant_kernel(const QuantPrefillArgs p) {
   bool failed = __syncthreads_or(!arrived);
   if (n_tiles > 0 && !failed) convert(0);
   __syncthreads();
-  for (int i = 0; i < n_tiles && !failed; ++i) {
+  int i = 0;
+  for (; i < n_tiles && !failed; ++i) {
     if (warp == 0 && i + 2 < n_tiles) {
       if ((i + 2) % 32 == 0) my_page = page_of(i + 2 + lane);
       issue(i + 2);
@@ -298,8 +299,8 @@ attn_prefill_quant_kernel(const QuantPrefillArgs p) {
   }
   if (failed) {   // a copy did not arrive: report, wait (again within bounds) for what else is on its way, and make the rows unmistakably wrong
     if (threadIdx.x == 0 && p.err) atomicOr(p.err, ERR_WAIT_TIMEOUT);
-    aq_wait(aq_smem(&bars[0]), 0);
-    aq_wait(aq_smem(&bars[1]), 0);
+    const int issued = min(n_tiles, i + QP_STAGES);     // (an iteration issues one tile, and the first two were before them)
+    for (int k = max(0, issued - QP_STAGES); k < issued; ++k) aq_wait(aq_smem(&bars[k % QP_STAGES]), k / QP_STAGES & 1);
     ma = mb = 0.f;
     la = lb = CUDART_NAN_F;
   }
