@@ -1600,14 +1600,14 @@ def _quant_cache(kcache, vcache, k_scale, v_scale, nkv, hd, what):
 def _quant_steps(page_table, tensors, device, what):
     """Checks the page table and the (tensor, least count) pairs; the table as the kernels read it, and its pitch: the kernels look up
     no page behind the pitch, so it has to be the width, and a view whose rows lie otherwise is laid out anew."""
-    stride, shape = page_table.stride(), page_table.shape
-    if len(stride) != 2 or (stride[1] != 1 and shape[1] > 1) or page_table.dtype != torch.int32 or page_table.get_device() != device:
+    shape = page_table.shape
+    if len(shape) != 2 or page_table.dtype != torch.int32 or page_table.get_device() != device or not (page_table.is_contiguous() or page_table.stride(1) == 1):
         raise KernelError(f"{what}: the page table must be int32 rows on the cache's device")
     for t, n in tensors:
         if t.dtype != torch.int32 or t.get_device() != device or not t.is_contiguous() or t.numel() < n:
             raise KernelError(f"{what}: positions, indices, tiles and the error word must be contiguous int32 tensors on the cache's device, one number each "
                               f"per token, sequence or tile (at least {n} here)")
-    return page_table if stride[0] == shape[1] or shape[0] == 1 else page_table.contiguous(), shape[1]
+    return page_table.contiguous(), shape[1]
 
 
 def _quant_tables(cos, sin, hd, device, what):
@@ -1765,12 +1765,14 @@ def attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_tabl
     keys = max_keys or page_table.shape[1] * PAGE
     if window > 0:
         keys = min(keys, window + most)
-    # (65,535 blocks along the grid's tiles; a block has at least 64 of a tile's rows of a kv head)
-    at_a_time = max(1, 65535 // max(1, -(-most * (nh // nkv) // 64)))
-    for first in range(0, n_tiles, at_a_time) if n_tiles > at_a_time else (0,):
-        tiles, ahead = min(at_a_time, n_tiles - first), 4 * first
-        _call_packed("edgelm_attn_prefill_quantized", 1 if n_tiles else 0, _QUANT_PREFILL,
-            qkv.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
-            tile_seq.data_ptr() + ahead, tile_tok0.data_ptr() + ahead, tile_ntok.data_ptr() + ahead, tile_pos0.data_ptr() + ahead,
-            err.data_ptr() if err is not None else 0, _raw_stream(device), ldq, ldo, _dt(qkv), code, pitch, n_pages, tiles, most, nh, nkv, hd, n_splits or 0, keys,
-            window, form, scale)
+    blocks = -(-most * (nh // nkv) // 64)                    # of a tile, a kv head's, at the most
+    if n_tiles * blocks > 65535 and 0 < 65535 // blocks < n_tiles:
+        for a in range(0, n_tiles, 65535 // blocks):         # (as many as a grid takes along its tiles)
+            tiles = [t.view(-1)[a:min(n_tiles, a + 65535 // blocks)] for t in (tile_seq, tile_tok0, tile_ntok, tile_pos0)]
+            attn_prefill_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, *tiles, tiles[0].numel(), nh, nkv, hd, scale, err, window,
+                                   max_keys, n_splits, form, most)
+        return
+    _call_packed("edgelm_attn_prefill_quantized", 1 if n_tiles else 0, _QUANT_PREFILL,
+        qkv.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(), seq_slot.data_ptr(),
+        tile_seq.data_ptr(), tile_tok0.data_ptr(), tile_ntok.data_ptr(), tile_pos0.data_ptr(), err.data_ptr() if err is not None else 0, _raw_stream(device),
+        ldq, ldo, _dt(qkv), code, pitch, n_pages, n_tiles, most, nh, nkv, hd, n_splits or 0, keys, window, form, scale)
