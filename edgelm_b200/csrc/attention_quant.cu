@@ -106,6 +106,7 @@ extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
   EL_REFUSE((uintptr_t)q % 16 == 0 && ldq % 4 == 0, "%s: query rows must start on a 16-byte boundary, a multiple of 4 numbers apart", who);
   EL_REFUSE((uintptr_t)out % 8 == 0 && ldo % 2 == 0, "%s: output rows must start on 8-byte boundaries", who);
   EL_REFUSE(form >= 0 && form <= 2, "%s: form %d", who, form);
+  EL_REFUSE(nkv <= 65535, "%s: %d key/value heads (takes up to 65,535)", who, nkv);
   // Sequences of one page stay on mma.sync: a block there starts sooner (us on mma.sync and tcgen05, 64 tokens: 9 heads of 64 on 3 5.6, 7.4; 16 of 128
   // on 4 6.9, 9.9; 16 sequences of 12 heads of 96 on 4 8.2, 11.6; 128 tokens: 7.6, 7.6; 9.5, 10.2; 15.7, 18.4, and of 9 heads of 64 9.3, 8.2).
   const bool taken = err != nullptr && prefill_quant_tc_takes(q, ldq, out, ldo, dtype, hd), tc = form == 2 ? taken : form == 0 && taken && max_keys > PAGE;
@@ -118,7 +119,7 @@ extern "C" int edgelm_attn_prefill_quantized(const QuantPrefillCall* call) {
     return 0;
   }
   const int per_tile = (max_tile_tokens * (nh / nkv) + QP_ROWS - 1) / QP_ROWS;
-  EL_REFUSE(nkv <= 65535 && (long long)n_tiles * per_tile <= 65535, "%s: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", who, n_tiles, per_tile);
+  EL_REFUSE((long long)n_tiles * per_tile <= 65535, "%s: %d tiles of %d blocks (takes up to 65,535 blocks a kv head)", who, n_tiles, per_tile);
   const QuantPrefillArgs p = {q, out, (const uint8_t*)kcache, (const uint8_t*)vcache, k_scale, v_scale, page_table, seq_slot, tile_seq, tile_tok0, tile_ntok,
                               tile_pos0, err, ldq, ldo, table_stride, n_pages, nh, nkv, window, per_tile, max_keys, scale};
   const int rc = format == QF_INT8 ? launch_prefill_quant_int8(p, dtype, hd, n_tiles, n_splits, stream) : launch_prefill_quant_fp8(p, dtype, hd, n_tiles, n_splits, stream);
