@@ -6,7 +6,8 @@
 // and sum   w_j c_j  with w_j = t_j f_j 2^-32 (the operand of the product with the codes: a float16 number under 2^15), and t_j 2^-e_j
 // (the same weight without its value's scale, in float32).  A weight is small beside the largest *weighted* row only, whatever the
 // scales of the rows, so no scale pushes the operand out of float16's range: 2^14 keeps 28 bits below the largest weight above
-// float16's smallest normal number (a key is off by 2^-39 of the largest weighted row at most, besides its operand's rounding), and where all rows' scales lie under 2^-60 (the format's smallest is 2^-67 or so) 11 bits are left down to
+// float16's smallest normal number (a key is off by 2^-39 of the largest weighted row at most, besides its operand's rounding; on tcgen05, whose M
+// lags behind the largest by up to 2^8 and whose operand is t 2^-40, 2^6 to 2^14 and 2^-31), and where all rows' scales lie under 2^-60 (the format's smallest is 2^-67 or so) 11 bits are left down to
 // 2^-87.  2^46 holds the other sum apart from both ends of float32: a term is at most 2^106, and rows drop out of it only where their
 // scale lies 150 powers of two or more under that of a row they compete with.  Taking e_j off the float is exact and costs no
 // logarithm.

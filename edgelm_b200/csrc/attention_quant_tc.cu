@@ -2,11 +2,11 @@
 // sizes up to 128.  The other head sizes, float32 models and sequences of one page stay on mma.sync (attention_quant_prefill.cuh).
 //
 // The tensor cores take float16 operands, so the codes become float16 on the chip.  Scales are applied 32 keys (a group) at a time: with
-// 2^k and 2^e the largest powers of two in the group's key and value scales, the tiles hold a_j (u_j / 2^k) and c_j (v_j / 2^e), one more
-// rounding to 11 bits each, and   x_ij = log2(e) scale 2^k (q_i . tile_j) + e,   t_ij = 2^(x_ij - M_i + 46),
+// 2^k and 2^e the largest powers of two in the group's key and value scales, the tiles hold a_j (u_j / 2^k) and c_j (v_j / 2^e), two more
+// roundings to 11 bits each (the factor u_j / 2^k, which all of a key's products share, and its product with a code), and   x_ij = log2(e) scale 2^k (q_i . tile_j) + e,   t_ij = 2^(x_ij - M_i + 46),
 // out_i = 2^40 sum (t_ij 2^-40) (tile_j) / sum t_ij 2^-e   (attention_quant.cuh, with one e a group).  A softmax thread has one group: two
 // numbers for 32 scores.  (Scales applied a key at a time cost a thread four shared-memory reads for four scores, 16 bytes to every lane
-// though all lanes read the same: 2,048 clocks a block of keys, twice its exponentials; 2,048 tokens of 32 heads of 64: 82 us, now 68.)
+// though all lanes read the same: 2,048 clocks a block of keys, twice its 1,024 of exponentials; 2,048 tokens of 32 heads of 64: 82 us, now 68.)
 // Where a group's key or value scales differ by more than 2^8 the tiles hold its codes as they are and the thread takes the slow way,
 // scales a key at a time: a row must not lose digits to a neighbour that it may not even see.  A row that is no number makes its key's
 // tile one of not-a-numbers (or, the slow way, its factor): who sees the key sees NaN, and only numbers enter the product with the values.
@@ -19,11 +19,11 @@
 // so that S of block j + 1 is computed beside the softmax of block j; the weights go back over the scores that they came from.
 // Few rows over many keys (a short turn of a long conversation): a cluster of up to 8 blocks shares a row tile's key blocks, and the partial
 // results meet in distributed shared memory in a fixed order.
-// Bound by the softmax: a block of 128 keys takes 3,050 clocks, of them 630 to read and find the maxima, 440 at the exchange between a row's
+// Bound by the softmax: a block of 128 keys takes 3,050 clocks (before the branch for scores far from zero, which costs 1 to 2 %), of them 630 to read and find the maxima, 440 at the exchange between a row's
 // threads, 1,280 for exponents, weights and sums, 305 waiting for S; the matrix products fill a sixth of it.  All 16 warps stand at the
 // same place; two teams of softmax warps on alternate blocks (28 warps, one block of keys behind the other) took 69.5 us for 68, and 88 for
 // 78 at a head size of 128: the registers of a thread then hold half of what they do now.  2,048 tokens of 32 heads of 64, e4m3: 68 us, 253
-// TFLOP/s by the products that the mask leaves; four turns of 65 to 701 tokens behind 1,501, 16 heads of 128 on 4, int8: 81 us.
+// TFLOP/s by the products that the mask leaves; four turns of 65 to 701 tokens behind 1,501, 16 heads of 128 on 4, int8: 82 us.
 // Every wait is bounded; where one runs out the block reports it, writes not-a-numbers and waits for what it has in flight before
 // it gives its memory back.
 #include <cooperative_groups.h>

@@ -1676,8 +1676,9 @@ def quantized_rows(kcache, vcache, k_scale, v_scale, tok_pos, tok_seq, seq_slot,
 
 
 def quantized_decode_splits(n_seqs, nh, nkv, hd, max_keys, n_sms=148):
-    """Blocks that share a sequence's keys in the decode attention over the 8-bit cache: what one wave of blocks of eight warps, one an SM,
-    leaves free, as long as each warp can get a tile of keys (64, 32 or 16 by head size).  A quarter of the SMs stays out of the count:
+    """Blocks that share a sequence's keys in the decode attention over the 8-bit cache: what one wave of blocks, one an SM,
+    leaves free, as long as eight of a block's warps can get a tile of keys each (64, 32 or 16 by head size; a grid of so few blocks is launched
+    with twelve a block, of which the last four may then have none).  A quarter of the SMs stays out of the count:
     clusters of 8 lie within a GPC, and 16 of them did not all find room at a time (16 heads on 4 of 128, 65,001 keys: 96 blocks 28 us,
     128 blocks 43)."""
     blocks = n_seqs * nkv * -(-(nh // nkv) // 8)
@@ -1737,7 +1738,8 @@ def attn_decode_quantized(q, out, kcache, vcache, k_scale, v_scale, page_table, 
 def attn_decode_rope_quantized(qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv, hd, scale,
                                n_splits=None, err=None, window=0, meta_ready=False, scratch=None):
     """`attn_decode_quantized` with the rotation and the append fused in: `qkv` holds the raw projections of one new token per sequence;
-    the rotated keys and the values are written into the cache as codes, the same as `rope_quantize_append` writes."""
+    the rotated keys and the values are written into the cache as codes, the same as `rope_quantize_append` writes.  A sequence (its pages)
+    comes at most once a call: what one token of it appends, another would read or not."""
     _need(cos is not None and sin is not None, "attn_decode_rope_quantized: needs the position table")
     _attn_decode_quantized("attn_decode_rope_quantized", qkv, out, kcache, vcache, k_scale, v_scale, page_table, seq_slot, seq_pos, cos, sin, n_seqs, nh, nkv,
                            hd, scale, n_splits, err, window, meta_ready, scratch)
