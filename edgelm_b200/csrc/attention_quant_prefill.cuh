@@ -241,12 +241,18 @@ attn_prefill_quant_kernel(const QuantPrefillArgs p) {
       la *= fa;
       lb *= fb;
       float ba = AQ_LIFT - ref_a, bb = AQ_LIFT - ref_b;
-      if (fmaxf(fabsf(ref_a), fabsf(ref_b)) > AQ_FAR) {
-        ba = bb = AQ_LIFT;
+      if (fabsf(ref_a) > AQ_FAR) {     // (each row by itself: no row's bits hang on another's)
+        ba = AQ_LIFT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           s[nt][0] -= ref_a;
           s[nt][1] -= ref_a;
+        }
+      }
+      if (fabsf(ref_b) > AQ_FAR) {
+        bb = AQ_LIFT;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
           s[nt][2] -= ref_b;
           s[nt][3] -= ref_b;
         }

@@ -108,3 +108,18 @@ def test_large_keys_under_small_queries(kernel, dtype, nh, nkv, hd, splits):
     cache["ks"].mul_(2.0 ** (115 - torch.randint(0, 13, cache["ks"].shape, generator=g)).to(DEV))
     q = torch.randn((n, nh, hd), generator=g).to(DTYPES[dtype]).to(DEV) * 2.0 ** -98
     check_one_key_takes_all(kernel, q, cache, table, total, nh, nkv, hd, 1 / math.sqrt(hd), splits)
+
+
+@pytest.mark.parametrize("kernel,dtype,nh,nkv,hd,splits", KERNELS)
+def test_rows_far_from_zero_stay_to_themselves(kernel, dtype, nh, nkv, hd, splits):
+    """Rows whose scores are far from zero (a query 2^14 or 2^60 times as large) beside usual ones: the usual ones' bits do not change."""
+    total, n = 300, 70
+    cache, table = ref.make_cache("int8", nkv, hd, [total], DEV, 3)
+    q = torch.randn((n, nh, hd), generator=torch.Generator().manual_seed(5)).to(DTYPES[dtype]).to(DEV)
+    large, hit = q.clone(), torch.zeros((n, nh), dtype=torch.bool, device=DEV)
+    for i, (t, h) in enumerate([(0, 0), (3, nh - 1), (9, 1), (40, 0), (69, nh - 1)]):
+        large[t, h] *= 2.0 ** (14 if i % 2 else 60)
+        hit[t, h] = True
+    args = (cache, table, total, nh, nkv, hd, 1 / math.sqrt(hd), splits)
+    a, b = attend(kernel, q, *args), attend(kernel, large, *args)
+    assert torch.equal(a[~hit], b[~hit]) and bool((a[hit] != b[hit]).any()) and bool(b.isfinite().all())
