@@ -240,28 +240,11 @@ attn_prefill_quant_kernel(const QuantPrefillArgs p) {
       mb = xb;
       la *= fa;
       lb *= fb;
-      float ba = AQ_LIFT - ref_a, bb = AQ_LIFT - ref_b;
-      if (fabsf(ref_a) > AQ_FAR) {     // (each row by itself: no row's bits hang on another's)
-        ba = AQ_LIFT;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[nt][0] -= ref_a;
-          s[nt][1] -= ref_a;
-        }
-      }
-      if (fabsf(ref_b) > AQ_FAR) {
-        bb = AQ_LIFT;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[nt][2] -= ref_b;
-          s[nt][3] -= ref_b;
-        }
-      }
       uint32_t w[TERMS][NT][2];      // the weights as the A operand: rows gid and gid + 8, keys 2 tig and the next of every 8
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float2 k0 = *(reinterpret_cast<const float2*>(&kd[nt * 8 + 2 * tig]) + 1), k1 = *(reinterpret_cast<const float2*>(&kd[nt * 8 + 2 * tig + 1]) + 1);
-        const float t0 = aq_exp2(s[nt][0] + ba), t1 = aq_exp2(s[nt][1] + ba), t2 = aq_exp2(s[nt][2] + bb), t3 = aq_exp2(s[nt][3] + bb);
+        const float t0 = aq_exp2(s[nt][0] - ref_a + AQ_LIFT), t1 = aq_exp2(s[nt][1] - ref_a + AQ_LIFT), t2 = aq_exp2(s[nt][2] - ref_b + AQ_LIFT), t3 = aq_exp2(s[nt][3] - ref_b + AQ_LIFT);
         la = fmaf(t0, k0.y, fmaf(t1, k1.y, la));
         lb = fmaf(t2, k0.y, fmaf(t3, k1.y, lb));
         float w0 = t0 * k0.x, w1 = t1 * k1.x, w2 = t2 * k0.x, w3 = t3 * k1.x;
