@@ -11,7 +11,7 @@
 // tile, by one lane, and not by all that use them.
 //
 // 64 sequences of 700 to 2,300 keys, 32 heads of 64: 87 us int8, 79 us e4m3 for 419 MB (4.8 and 5.3 TB/s; the floor is 64 us).  There the
-// warps' instructions bound it (866 a tile of 64 keys, 376 of them on the ALU pipe, most of these the codes' way to float16; ncu: issue
+// warps' instructions bound it (about 870 a tile of 64 keys, 376 of them on the ALU pipe, most of these the codes' way to float16; ncu: issue
 // slots 47 % busy with 9 warps an SM, as many as the stages leave room for); shorter stages make room for twice the warps and need more
 // instructions a key: 83 to 92 us.
 //
